@@ -77,9 +77,28 @@ class TilingInfo(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class Strides(ctypes.Structure):
+    """fa_strides: elements between batch entries, heads and rows."""
+
+    _fields_ = [(name, ctypes.c_longlong) for name in ("batch", "head", "row")]
+
+
+class PagedCacheInfo(ctypes.Structure):
+    """fa_paged_cache."""
+
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("k", "v")]
+                + [(name, ctypes.c_longlong) for name in ("block_stride", "head_stride", "token_stride")]
+                + [(name, ctypes.c_int) for name in ("num_blocks", "heads_kv", "block_size", "head_dim", "dtype")])
+
+
 # Every symbol include/fa_mi355x.h declares, with its ctypes signature.
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
+_ll = ctypes.c_longlong
+_sz = ctypes.c_size_t
+_strides = ctypes.POINTER(Strides)
+_cache = ctypes.POINTER(PagedCacheInfo)
+_ip = ctypes.POINTER(_i)
 _SIGNATURES = {
     "fa_get_last_error": (_i, []),
     "fa_peek_at_last_error": (_i, []),
@@ -113,6 +132,15 @@ _SIGNATURES = {
                            ctypes.POINTER(ctypes.c_float), _vp]),
     "fa_mfma_peak_records_bytes": (ctypes.c_size_t, []),
     "fa_mfma_peak": (_i, [_vp, _i, _i, _vp, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double), _vp]),
+    "fa_launch_paged_slots": (_i, [_vp] * 8 + [_i, _i, _ll, _i, _i, _i, _vp]),
+    "fa_launch_paged_append": (_i, [_vp, _vp, _vp, _cache, _i, _strides, _strides, _vp]),
+    "fa_attention_paged_workspace_bytes": (_sz, [_i] * 7),
+    "fa_attention_paged_config": (_i, [_i] * 7 + [_ip, _ip]),
+    "fa_launch_attention_paged": (_i, [_vp, _cache, _vp, _vp, _sz, _vp, _vp, _vp, _i, _i, _i, _i, _ll, _i, _i, _i,
+                                       _strides, _strides, _vp]),
+    "fa_attention_cross_workspace_bytes": (_sz, [_i] * 6),
+    "fa_attention_cross_config": (_i, [_i] * 6 + [_ip, _ip]),
+    "fa_launch_attention_cross": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _vp] + [_i] * 7 + [_strides] * 4 + [_vp]),
     "fa_build_info": (ctypes.c_char_p, []),
 }
 
@@ -470,3 +498,10 @@ def attention_forward(q, k, v, causal: bool = False, kernel: str = "v3_mfma", ou
     else:
         raise ValueError(f"unknown kernel {kernel!r}")
     return o
+
+
+from .serving import (  # noqa: E402
+    DTYPE_BF16, DTYPE_FP16, PagedCache, PagedSlots, attention_cross, attention_cross_config, attention_cross_workspace,
+    attention_cross_workspace_bytes, attention_paged, attention_paged_config, attention_paged_workspace,
+    attention_paged_workspace_bytes, launch_attention_cross, launch_attention_paged, launch_paged_append,
+    launch_paged_slots, paged_append, paged_cache, paged_slots, paged_slots_buffers)

@@ -1,0 +1,731 @@
+// Attention for serving: new tokens over a paged K/V cache, and queries over an
+// encoder's states of another length. One kernel computes both; they differ in
+// where the rows of a sequence and its keys lie.
+//
+//   O[i] = sum_j P_ij V_j / sum_j P_ij,  P_ij = exp(q_i . k_j / sqrt(D) - m_i),
+//
+// over the keys j < limit(i). The running base m_i and sum stay in 32 bits; the
+// weights are rounded to the element type for the second matrix product (half a
+// step of 16 bits each, as in the fused self-attention), and their sum uses the
+// rounded values.
+//
+// Work: the query heads that share a key head are packed beside each other, row
+// r of a sequence is token r / group and head r % group of the key head, so K and
+// V are read once for all of them. A workgroup owns 32 * kWaves rows of one key
+// head (a wave owns 32) and walks 32-key tiles that its waves copy HBM -> LDS
+// together. Few rows over many keys leave the device idle, so the keys of a row
+// block are split into chunks over workgroups; their partial results (O, base, sum
+// in 32 bits) are joined by a second kernel.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "fa_paged.hpp"
+#include "fa_serving_core.hpp"
+
+namespace {
+
+using namespace fa::serving;
+using fa::f32x16;
+using fa::f32x4;
+using fa::i32x4;
+
+constexpr int kMaxSplits = 256;
+constexpr long long kMaxKeys = 1LL << 30;  // of one sequence
+constexpr long long kMaxRows = 1LL << 30;  // of one sequence and key head
+
+// One launch. Strides and offsets are in elements.
+struct Args
+{
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* o;
+    float* part;         // [row][split][D] of the split launches
+    float* base_sum;     // [row][split][2]
+    const int* table;    // paged: block table
+    const int* starts;   // paged: first token of each sequence
+    const int* lens;     // keys of each sequence (may be null where not paged)
+    long long q_seq, q_head, q_row;
+    long long o_seq, o_head, o_row;
+    long long k_seq, k_head, k_row;  // k_seq: from page to page, or from sequence to sequence
+    long long v_seq, v_head, v_row;
+    long long table_stride;
+    int table_width, num_blocks, block_shift;
+    int seqs, tokens, heads_kv, group, max_queries, max_keys;
+    int slots;      // row blocks of a key head over all sequences
+    int per_seq;    // row blocks per sequence; 0: found from `starts`
+    int splits, chunk;
+    int causal;
+    float c_log2;   // log2(e) / sqrt(D)
+};
+
+// What a row block works on.
+struct Block
+{
+    int seq, head;       // sequence, key head
+    int row0, rows;      // first row within the sequence, rows of the sequence
+    int first_token;     // paged: the sequence's first row of q
+    int keys;            // keys in reach
+    int shift;           // token i sees the keys below shift + i + 1 (causal)
+    int end;             // keys that the block's last row sees
+    int splits;          // chunks of those keys
+};
+
+__device__ __forceinline__ int limit_of(const Args& a, const Block& b, int token)
+{
+    return a.causal ? max(0, min(b.keys, b.shift + token + 1)) : b.keys;
+}
+
+// The block of `slot` (of R rows). False: it holds no row.
+template <int R, bool kPaged>
+__device__ __forceinline__ bool find_block(const Args& a, int slot, int head, Block& b)
+{
+    int rb, tokens;
+    b.head = head;
+    if constexpr (kPaged)
+    {
+        auto start_of = [&](int s) { return max(0, min(a.starts[s], a.tokens)); };
+        if (a.per_seq > 0)
+        {
+            b.seq = slot / a.per_seq;
+            rb = slot % a.per_seq;
+        }
+        else
+        {
+            // Sequence s owns the slots from floor(first row / R) + s on, at least
+            // as many as it has blocks. The first slots of 64 sequences are
+            // compared at a time, each time one 64th of those left.
+            const int lane = threadIdx.x & 63;
+            int lo = 0, hi = a.seqs;
+            auto first_slot = [&](int s) {
+                return static_cast<int>(static_cast<long long>(start_of(s)) * a.group / R) + s;
+            };
+            while (hi - lo > 1)
+            {
+                const int step = (hi - lo + 63) / 64;
+                const int s = lo + lane * step;
+                const bool below = s < hi && first_slot(s) <= slot;
+                const int count = max(1, __popcll(__ballot(below)));
+                lo += (count - 1) * step;
+                hi = min(hi, lo + step);
+            }
+            b.seq = uniform(lo);
+            rb = slot - uniform(first_slot(b.seq));
+        }
+        b.first_token = uniform(start_of(b.seq));
+        tokens = max(0, uniform(start_of(b.seq + 1)) - b.first_token);
+        const int len = max(0, uniform(a.lens[b.seq]));
+        b.keys = static_cast<int>(min(static_cast<long long>(len), static_cast<long long>(a.table_width) << a.block_shift));
+        b.shift = len - tokens;
+        b.rows = min(tokens, a.max_queries) * a.group;
+    }
+    else
+    {
+        b.seq = slot / a.per_seq;
+        rb = slot % a.per_seq;
+        b.first_token = 0;
+        b.keys = a.lens ? max(0, min(uniform(a.lens[b.seq]), a.max_keys)) : a.max_keys;
+        b.shift = 0;
+        b.rows = a.max_queries * a.group;
+    }
+    if (rb < 0 || static_cast<long long>(rb) * R >= b.rows) return false;
+    b.row0 = rb * R;
+    b.end = limit_of(a, b, (min(b.row0 + R, b.rows) - 1) / a.group);
+    b.splits = max(1, min(a.splits, (b.end + a.chunk - 1) / a.chunk));
+    return true;
+}
+
+// Row r's place among all rows of q (the partial results' rows).
+template <bool kPaged>
+__device__ __forceinline__ long long part_row(const Args& a, const Block& b, int token, int h)
+{
+    const long long t = kPaged ? static_cast<long long>(b.first_token) + token
+                               : static_cast<long long>(b.seq) * a.max_queries + token;
+    return t * (static_cast<long long>(a.heads_kv) * a.group) + b.head * a.group + h;
+}
+
+template <typename T, int D, int kWaves, bool kPaged>
+__global__ __launch_bounds__(64 * kWaves) void serving_attention_kernel(const Args a)
+{
+    using E = Elem<T>;
+    using x8 = typename E::x8;
+    using C = TileCopy<D, kWaves>;
+    constexpr int R = 32 * kWaves;
+    constexpr int kStages = 3;
+    constexpr int kTile = kTileKeys * D;  // elements
+    __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStages * kTile];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int i = lane & 31;
+    const int h = lane >> 5;
+
+    const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.heads_kv));
+    const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.heads_kv));
+    const int split = rest % a.splits;
+    // Late rows see the most keys: they start first.
+    const int slot = a.slots - 1 - rest / a.splits;
+    Block b;
+    if (!find_block<R, kPaged>(a, slot, head, b)) return;
+    if (split >= b.splits) return;
+
+    // The lane's row; lanes past the last row repeat it and store nothing.
+    const int row = b.row0 + 32 * wave + i;
+    const int row_in = min(row, b.rows - 1);
+    const int token = row_in / a.group;
+    const int qh = row_in % a.group;
+    const int limit = limit_of(a, b, token);
+
+    const int k_begin = split * a.chunk;
+    const int k_end = split == b.splits - 1 ? b.end : k_begin + a.chunk;
+    const int t_begin = k_begin / kTileKeys;
+    const int t_end = (k_end + kTileKeys - 1) / kTileKeys;  // == t_begin where nothing is seen
+    // Tiles of this wave: up to its last row's limit, masked from its first row's on.
+    const int row_last = min(b.row0 + 32 * wave + 31, b.rows - 1);
+    const int wave_end = b.row0 + 32 * wave < b.rows ? limit_of(a, b, row_last / a.group) : 0;
+    const int t_last = min(t_end, (wave_end + kTileKeys - 1) / kTileKeys);
+    const int t_mask = limit_of(a, b, min(b.row0 + 32 * wave, b.rows - 1) / a.group) / kTileKeys;
+
+    // Byte offset of 16 keys from `key` on, and the bytes of them that exist: a
+    // copy's rows past those read as zero, and so does a page that the cache
+    // does not have.
+    const uint32_t k_row_bytes = static_cast<uint32_t>(a.k_row * 2);
+    const uint32_t v_row_bytes = static_cast<uint32_t>(a.v_row * 2);
+    int pages = 0, pages_base = -1;  // lane l: entry pages_base + l of the block table
+    const uint64_t k_bytes = uniform(reinterpret_cast<uint64_t>(a.k) + static_cast<uint64_t>(b.head * a.k_head * 2) +
+                                     (kPaged ? 0 : static_cast<uint64_t>(b.seq * a.k_seq * 2)));
+    const uint64_t v_bytes = uniform(reinterpret_cast<uint64_t>(a.v) + static_cast<uint64_t>(b.head * a.v_head * 2) +
+                                     (kPaged ? 0 : static_cast<uint64_t>(b.seq * a.v_seq * 2)));
+    struct Half
+    {
+        uint64_t k, v;
+        int rows;
+    };
+    auto half_at = [&](int key) {
+        Half r;
+        r.rows = max(0, min(16, b.end - key));
+        if constexpr (kPaged)
+        {
+            const int entry = key >> a.block_shift;
+            if ((entry & ~63) != pages_base)
+            {
+                pages_base = entry & ~63;
+                const int e = pages_base + lane;
+                pages = e < a.table_width ? a.table[b.seq * a.table_stride + e] : -1;
+            }
+            const int page = __builtin_amdgcn_readlane(pages, entry & 63);
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_blocks)) r.rows = 0;
+            const long long in_page = key & ((1 << a.block_shift) - 1);
+            const long long p = r.rows ? page : 0;
+            r.k = k_bytes + static_cast<uint64_t>((p * a.k_seq + in_page * a.k_row) * 2);
+            r.v = v_bytes + static_cast<uint64_t>((p * a.v_seq + in_page * a.v_row) * 2);
+        }
+        else
+        {
+            r.k = k_bytes + static_cast<uint64_t>(key * a.k_row * 2);
+            r.v = v_bytes + static_cast<uint64_t>(key * a.v_row * 2);
+        }
+        return r;
+    };
+    auto descriptor = [&](uint64_t base, int rows, uint32_t row_bytes) {
+        i32x4 r;
+        r[0] = uniform(static_cast<int>(static_cast<uint32_t>(base)));
+        r[1] = uniform(static_cast<int>(static_cast<uint32_t>(base >> 32) & 0xffffu));
+        r[2] = uniform(rows > 0 ? static_cast<int>((rows - 1) * row_bytes + D * 2) : 0);
+        r[3] = static_cast<int>(fa::kRawBufferConfig);
+        return r;
+    };
+    // A copy's lanes: row and chunk of each lane's 16 bytes, from the half's first row.
+    uint32_t koff[C::kIssues], voff[C::kIssues];
+    {
+        const int sub = (lane % C::kLanes) / C::kChunks;
+        const int pchunk = lane % C::kChunks;
+#pragma unroll
+        for (int u = 0; u < C::kIssues; ++u)
+        {
+            const int r = (u * kWaves + wave) * C::kRows + sub;
+            koff[u] = static_cast<uint32_t>(r & 15) * k_row_bytes + ((pchunk ^ swz_k<D>(r)) * 16);
+            voff[u] = static_cast<uint32_t>(r & 15) * v_row_bytes + ((pchunk ^ swz_v<D>(r)) * 16);
+        }
+    }
+    const uint32_t lds_base = fa::lds_addr(lds);
+    auto copy_tile = [&](int t) {
+        const int stage = t % kStages;
+        const Half lo = half_at(t * kTileKeys), hi = half_at(t * kTileKeys + 16);
+#pragma unroll
+        for (int u = 0; u < C::kIssues; ++u)
+        {
+            const int r0 = (u * kWaves + wave) * C::kRows;
+            const uint64_t kb = r0 < 16 ? lo.k : hi.k, vb = r0 < 16 ? lo.v : hi.v;
+            const int rows = r0 < 16 ? lo.rows : hi.rows;
+            const uint32_t at = lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes;
+            const i32x4 kd = descriptor(kb, rows, k_row_bytes);
+            const i32x4 vd = descriptor(vb, rows, v_row_bytes);
+            if (C::kLanes == 64 || lane < C::kLanes)
+            {
+                fa::dma16(kd, koff[u], at);
+                fa::dma16(vd, voff[u], at + kStages * kTile * 2);
+            }
+        }
+    };
+
+    copy_tile(t_begin);
+    copy_tile(t_begin + 1);
+
+    x8 qr[D / 16];
+    {
+        const uint16_t* qp = a.q + (kPaged ? (b.first_token + static_cast<long long>(token)) * a.q_row
+                                           : b.seq * a.q_seq + token * a.q_row) +
+                             (b.head * a.group + qh) * a.q_head;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qr[ks] = *reinterpret_cast<const x8*>(qp + 16 * ks + 8 * h);
+    }
+    int k_at[D / 16], v_at[D / 32];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) k_at[ks] = i * D + (((2 * ks + h) ^ swz_k<D>(i)) << 3);
+    {
+        const int g16 = lane >> 4, s16 = lane & 15;
+        const int vr = 4 * (g16 >> 1) + (s16 >> 2);
+        const int dim = 16 * (g16 & 1) + 4 * (s16 & 3);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+        {
+            const int col = 32 * db + dim;
+            v_at[db] = kStages * kTile + vr * D + (((col >> 3) ^ swz_v<D>(vr)) << 3) + (col & 7);
+        }
+    }
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+    float m = kEmptyBase, l = 0.0f;
+
+    for (int t = t_begin; t < t_end; ++t)
+    {
+        // Tile t has landed once only tile t+1's copies are in flight; past the
+        // barrier every wave has left tile t-1, whose stage takes tile t+2.
+        fa::wait_vm_lgkm0<2 * C::kIssues>();
+        barrier();
+        copy_tile(t + 2);
+        if (t >= t_last) continue;
+        const uint16_t* const stage = lds + (t % kStages) * kTile;
+        f32x16 s = {};
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) s = E::mfma(*reinterpret_cast<const x8*>(stage + k_at[ks]), qr[ks], s);
+        if (t >= t_mask) mask_tile(s, limit - t * kTileKeys - 4 * h);
+        const float m_new = __builtin_elementwise_maximum(m, row_max_raw(s) * a.c_log2 - E::kBias);
+        if (__any(m_new != m))
+        {
+            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+            m = m_new;
+        }
+        x8 p[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+        {
+#pragma clang fp contract(off)
+            // The product is rounded as the base was: the largest score's weight
+            // is exactly 2^kBias however large the score.
+            const float x = s[r] * a.c_log2 - m;
+            p[r >> 3][r & 7] = static_cast<T>(__builtin_amdgcn_exp2f(x));
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) l = E::add_pair(p[r >> 3][r & 7], p[r >> 3][(r & 7) + 1], l);
+#pragma unroll
+        for (int mm = 0; mm < 2; ++mm)
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+            {
+                const uint16_t* base = stage + v_at[db] + mm * 16 * D;
+                const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base));
+                const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + 8 * D));
+                o[db] = E::mfma(__builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), p[mm],
+                                o[db]);
+            }
+    }
+    fa::wait_vm_lgkm0<0>();  // the last copies have landed before the workgroup's LDS goes
+
+    float la, lb;
+    row_halves(l, la, lb);
+    l = la + lb;
+    if (row >= b.rows) return;
+    if (b.splits > 1)
+    {
+        const long long pr = part_row<kPaged>(a, b, token, qh) * a.splits + split;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(a.part + pr * D + 32 * db + 8 * g + 4 * h) =
+                    f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+        if (h == 0)
+        {
+            a.base_sum[2 * pr] = m;
+            a.base_sum[2 * pr + 1] = l;
+        }
+        return;
+    }
+    // A row that saw nothing has the sum 0 and gives 0; a NaN sum leaves O's NaN.
+    const float inv = l > 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f;
+    uint16_t* op = a.o + (kPaged ? (b.first_token + static_cast<long long>(token)) * a.o_row
+                                 : b.seq * a.o_seq + token * a.o_row) +
+                   (b.head * a.group + qh) * a.o_head;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+        {
+            uint2 w;
+            w.x = pack_pair<T>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv);
+            w.y = pack_pair<T>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
+            *reinterpret_cast<uint2*>(op + 32 * db + 8 * g + 4 * h) = w;
+        }
+}
+
+// Joins the chunks of one row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c
+// with M the largest base. A workgroup per row; D/4 lanes read a chunk's 4 D
+// bytes, so 256 threads have 1024/D chunks in flight at a time.
+template <typename T, int D, int R, bool kPaged>
+__global__ __launch_bounds__(256) void serving_join_kernel(const Args a, int block_rows)
+{
+    constexpr int kLanes = D / 4;
+    constexpr int kAtOnce = 256 / kLanes;
+    __shared__ float weight[kMaxSplits];
+    __shared__ f32x4 sums[256];
+    const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.heads_kv));
+    const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.heads_kv));
+    Block b;
+    if (!find_block<R, kPaged>(a, rest / block_rows, head, b)) return;
+    const int row = b.row0 + rest % block_rows;
+    if (b.splits == 1 || row >= b.rows) return;
+    const int token = row / a.group, qh = row % a.group;
+    const long long pr = part_row<kPaged>(a, b, token, qh) * a.splits;
+
+    const int tid = threadIdx.x;
+    // Every wave finds the base and the sum for itself; wave 0 keeps the weights.
+    float top = kEmptyBase, total = 0.0f;
+    float mv[kMaxSplits / 64], lv[kMaxSplits / 64];
+#pragma unroll
+    for (int x = 0; x < kMaxSplits / 64; ++x)
+    {
+        const int c = 64 * x + (tid & 63);
+        mv[x] = kEmptyBase;
+        lv[x] = 0.0f;
+        if (c < b.splits)
+        {
+            mv[x] = a.base_sum[2 * (pr + c)];
+            lv[x] = a.base_sum[2 * (pr + c) + 1];
+        }
+        top = __builtin_elementwise_maximum(top, mv[x]);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, off, 64));
+#pragma unroll
+    for (int x = 0; x < kMaxSplits / 64; ++x)
+    {
+        const float w = __builtin_amdgcn_exp2f(mv[x] - top);
+        total += w * lv[x];
+        if (tid < 64) weight[64 * x + tid] = w;
+    }
+    total = fa::wave_sum(total);
+    __syncthreads();
+
+    f32x4 acc = {};
+    const int d4 = (tid % kLanes) * 4;
+#pragma unroll 4
+    for (int c = tid / kLanes; c < b.splits; c += kAtOnce)
+        acc += *reinterpret_cast<const f32x4*>(a.part + (pr + c) * D + d4) * weight[c];
+    sums[tid] = acc;
+    __syncthreads();
+    if (tid >= kLanes) return;
+#pragma unroll
+    for (int x = 1; x < kAtOnce; ++x) acc += sums[x * kLanes + tid];
+    const float inv = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
+    uint16_t* op = a.o + (kPaged ? (b.first_token + static_cast<long long>(token)) * a.o_row
+                                 : b.seq * a.o_seq + token * a.o_row) +
+                   (b.head * a.group + qh) * a.o_head;
+    uint2 w;
+    w.x = pack_pair<T>(acc[0] * inv, acc[1] * inv);
+    w.y = pack_pair<T>(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2*>(op + d4) = w;
+}
+
+// ---------------------------------------------------------------- host side
+
+// Rows of a workgroup, row blocks and key chunks of a launch.
+struct Plan
+{
+    int waves;
+    int per_seq;
+    long long slots;
+    int splits, chunk;
+    size_t workspace;
+};
+
+Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int head_dim, int max_queries, int max_keys,
+               bool paged)
+{
+    Plan p{};
+    max_keys = static_cast<int>(std::min<long long>(max_keys, kMaxKeys));
+    const int group = heads / heads_kv;
+    const long long rows = static_cast<long long>(std::min<long long>(max_queries, tokens)) * group;
+    p.waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    const int R = 32 * p.waves;
+    const long long per_seq = (rows + R - 1) / R;
+    p.per_seq = static_cast<int>(per_seq);
+    p.slots = seqs * per_seq;
+    // Ragged batches: at most one slot per full block of rows and one per sequence.
+    const long long packed = tokens * group / R + seqs;
+    if (paged && per_seq > 1 && packed < p.slots)
+    {
+        p.per_seq = 0;
+        p.slots = packed;
+    }
+    const long long blocks = p.slots * heads_kv;
+    const long long cus = fa::device_compute_units();
+    const long long target = cus * (p.waves == 1 ? 6 : p.waves == 2 ? 4 : p.waves == 4 ? 2 : 1);
+    const long long least = 256;  // keys per chunk
+    long long splits = std::max<long long>(1, std::min<long long>({target / std::max<long long>(1, blocks),
+                                                                   (max_keys + least - 1) / least, kMaxSplits}));
+    p.chunk = static_cast<int>(((max_keys + splits - 1) / splits + kTileKeys - 1) / kTileKeys * kTileKeys);
+    p.chunk = std::max(p.chunk, kTileKeys);
+    p.splits = static_cast<int>(std::max<long long>(1, (max_keys + static_cast<long long>(p.chunk) - 1) / p.chunk));
+    if (p.splits > 1) p.workspace = static_cast<size_t>(tokens) * heads * p.splits * (head_dim + 2) * sizeof(float);
+    return p;
+}
+
+template <typename T, int D, int kWaves, bool kPaged>
+int launch_typed(const Args& a, const Plan& p, int head_rows, hipStream_t stream)
+{
+    const long long blocks = p.slots * a.heads_kv * p.splits;
+    if (blocks > 0x7fffffffLL / (64 * kWaves)) return hipErrorInvalidValue;
+    const int block_rows = std::min(32 * kWaves, head_rows);
+    const long long join_blocks = p.slots * a.heads_kv * block_rows;
+    if (p.splits > 1 && join_blocks > 0x7fffffffLL / 256) return hipErrorInvalidValue;
+    hipError_t e = fa::launch_kernel(serving_attention_kernel<T, D, kWaves, kPaged>, dim3(static_cast<unsigned>(blocks)),
+                                     dim3(64 * kWaves), stream, a);
+    if (e != hipSuccess || p.splits == 1) return e;
+    return fa::launch_kernel(serving_join_kernel<T, D, 32 * kWaves, kPaged>, dim3(static_cast<unsigned>(join_blocks)),
+                             dim3(256), stream, a, block_rows);
+}
+
+template <typename T, int D, bool kPaged>
+int launch_waves(const Args& a, const Plan& p, int head_rows, hipStream_t stream)
+{
+    switch (p.waves)
+    {
+        case 1: return launch_typed<T, D, 1, kPaged>(a, p, head_rows, stream);
+        case 2: return launch_typed<T, D, 2, kPaged>(a, p, head_rows, stream);
+        case 4: return launch_typed<T, D, 4, kPaged>(a, p, head_rows, stream);
+        default: return launch_typed<T, D, 8, kPaged>(a, p, head_rows, stream);
+    }
+}
+
+template <bool kPaged>
+int launch_any(const Args& a, const Plan& p, int head_rows, int head_dim, int dtype, hipStream_t stream)
+{
+    if (dtype == FA_DTYPE_BF16)
+        return head_dim == 64 ? launch_waves<__bf16, 64, kPaged>(a, p, head_rows, stream)
+                              : launch_waves<__bf16, 128, kPaged>(a, p, head_rows, stream);
+    return head_dim == 64 ? launch_waves<_Float16, 64, kPaged>(a, p, head_rows, stream)
+                          : launch_waves<_Float16, 128, kPaged>(a, p, head_rows, stream);
+}
+
+// Rows are read and written in pieces of 16 bytes: every stride keeps them aligned.
+bool bad_strides(const fa_strides& s, bool with_batch)
+{
+    return ((with_batch ? s.batch : 0) | s.head | s.row) & 7;
+}
+
+// K and V: rows of a copy lie within 32-bit offsets of its first one, in rising order.
+bool bad_key_row(long long row, int head_dim) { return row < head_dim || row >= (1LL << 26); }
+
+int launch_paged(const void* q, const fa_paged_cache* cache, void* o, void* workspace, size_t workspace_bytes,
+                 const int* block_table, long long table_stride, int table_width, const int* query_starts,
+                 const int* kv_lens, int num_seqs, int tokens, int heads, int max_query_len, int max_kv_len, int causal,
+                 const fa_strides* q_strides, const fa_strides* o_strides, void* stream)
+{
+    if (!cache) return hipErrorInvalidValue;
+    if (cache->head_dim != 64 && cache->head_dim != 128) return FA_ERROR_UNSUPPORTED;
+    const int D = cache->head_dim, heads_kv = cache->heads_kv;
+    if (num_seqs < 0 || tokens < 0 || heads < 0 || max_query_len < 0 || max_kv_len < 0) return hipErrorInvalidValue;
+    if (num_seqs == 0 || tokens == 0 || heads == 0 || max_query_len == 0) return hipSuccess;
+    const int status = fa::check_paged_cache(*cache);
+    if (status != hipSuccess) return status;
+    if (heads_kv == 0 || heads % heads_kv != 0 || heads > 65536) return hipErrorInvalidValue;
+    if (!q || !o || !query_starts || !kv_lens) return hipErrorInvalidValue;
+    if (static_cast<long long>(std::min(max_query_len, tokens)) * (heads / heads_kv) > kMaxRows ||
+        static_cast<long long>(table_width) * cache->block_size > kMaxKeys)
+        return hipErrorInvalidValue;
+    if (table_width < 0 || (table_width > 0 && !block_table) || table_stride < 0) return hipErrorInvalidValue;
+    const fa_strides qs = q_strides ? *q_strides : fa_strides{0, D, static_cast<long long>(heads) * D};
+    const fa_strides os = o_strides ? *o_strides : fa_strides{0, D, static_cast<long long>(heads) * D};
+    if (fa::misaligned16(q) || fa::misaligned16(o) || bad_strides(qs, false) || bad_strides(os, false)) return hipErrorInvalidValue;
+    const Plan p = make_plan(num_seqs, tokens, heads, heads_kv, D, max_query_len, max_kv_len, true);
+    if (p.workspace > 0 && (!workspace || workspace_bytes < p.workspace || fa::misaligned16(workspace)))
+        return hipErrorInvalidValue;
+    Args a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(cache->k);
+    a.v = static_cast<const uint16_t*>(cache->v);
+    a.o = static_cast<uint16_t*>(o);
+    a.part = static_cast<float*>(workspace);
+    a.base_sum = a.part + static_cast<size_t>(tokens) * heads * p.splits * D;
+    a.table = block_table;
+    a.starts = query_starts;
+    a.lens = kv_lens;
+    a.q_head = qs.head, a.q_row = qs.row;
+    a.o_head = os.head, a.o_row = os.row;
+    a.k_seq = a.v_seq = cache->block_stride;
+    a.k_head = a.v_head = cache->head_stride;
+    a.k_row = a.v_row = cache->token_stride;
+    a.table_stride = table_stride;
+    a.table_width = table_width;
+    a.num_blocks = cache->num_blocks;
+    a.block_shift = __builtin_ctz(cache->block_size);
+    a.seqs = num_seqs;
+    a.tokens = tokens;
+    a.heads_kv = heads_kv;
+    a.group = heads / heads_kv;
+    a.max_queries = max_query_len;
+    a.slots = static_cast<int>(p.slots);
+    a.per_seq = p.per_seq;
+    a.splits = p.splits;
+    a.chunk = p.chunk;
+    a.causal = causal != 0;
+    a.c_log2 = fa_default_scale(D) * fa::kLog2e;
+    const int head_rows = static_cast<int>(std::min<long long>(1 << 20, static_cast<long long>(std::min(max_query_len, tokens)) * a.group));
+    return launch_any<true>(a, p, head_rows, D, cache->dtype, static_cast<hipStream_t>(stream));
+}
+
+int launch_cross(const void* q, const void* k, const void* v, void* o, void* workspace, size_t workspace_bytes,
+                 const int* kv_lens, int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim, int dtype,
+                 const fa_strides* q_strides, const fa_strides* k_strides, const fa_strides* v_strides,
+                 const fa_strides* o_strides, void* stream)
+{
+    if (head_dim != 64 && head_dim != 128) return FA_ERROR_UNSUPPORTED;
+    if (batch < 0 || heads < 0 || heads_kv < 0 || q_len < 0 || kv_len < 0) return hipErrorInvalidValue;
+    if (dtype != FA_DTYPE_BF16 && dtype != FA_DTYPE_FP16) return hipErrorInvalidValue;
+    if (batch == 0 || heads == 0 || q_len == 0) return hipSuccess;
+    if (heads_kv == 0 || heads % heads_kv != 0 || heads > 65536) return hipErrorInvalidValue;
+    if (!q || !o || (kv_len > 0 && (!k || !v))) return hipErrorInvalidValue;
+    if (static_cast<long long>(q_len) * (heads / heads_kv) > kMaxRows || kv_len > kMaxKeys) return hipErrorInvalidValue;
+    auto contiguous = [&](int h, int n) {
+        return fa_strides{static_cast<long long>(h) * n * head_dim, static_cast<long long>(n) * head_dim, head_dim};
+    };
+    const fa_strides qs = q_strides ? *q_strides : contiguous(heads, q_len);
+    const fa_strides ks = k_strides ? *k_strides : contiguous(heads_kv, kv_len);
+    const fa_strides vs = v_strides ? *v_strides : contiguous(heads_kv, kv_len);
+    const fa_strides os = o_strides ? *o_strides : contiguous(heads, q_len);
+    if (fa::misaligned16(q) || fa::misaligned16(k) || fa::misaligned16(v) || fa::misaligned16(o)) return hipErrorInvalidValue;
+    if (bad_strides(qs, true) || bad_strides(ks, true) || bad_strides(vs, true) || bad_strides(os, true))
+        return hipErrorInvalidValue;
+    if (bad_key_row(ks.row, head_dim) || bad_key_row(vs.row, head_dim)) return hipErrorInvalidValue;
+    const long long tokens = static_cast<long long>(batch) * q_len;
+    const Plan p = make_plan(batch, tokens, heads, heads_kv, head_dim, q_len, kv_len, false);
+    if (p.slots > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (p.workspace > 0 && (!workspace || workspace_bytes < p.workspace || fa::misaligned16(workspace)))
+        return hipErrorInvalidValue;
+    Args a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.o = static_cast<uint16_t*>(o);
+    a.part = static_cast<float*>(workspace);
+    a.base_sum = a.part + static_cast<size_t>(tokens) * heads * p.splits * head_dim;
+    a.lens = kv_lens;
+    a.q_seq = qs.batch, a.q_head = qs.head, a.q_row = qs.row;
+    a.o_seq = os.batch, a.o_head = os.head, a.o_row = os.row;
+    a.k_seq = ks.batch, a.k_head = ks.head, a.k_row = ks.row;
+    a.v_seq = vs.batch, a.v_head = vs.head, a.v_row = vs.row;
+    a.seqs = batch;
+    a.heads_kv = heads_kv;
+    a.group = heads / heads_kv;
+    a.max_queries = q_len;
+    a.max_keys = kv_len;
+    a.slots = static_cast<int>(p.slots);
+    a.per_seq = p.per_seq;
+    a.splits = p.splits;
+    a.chunk = p.chunk;
+    a.c_log2 = fa_default_scale(head_dim) * fa::kLog2e;
+    const int head_rows = static_cast<int>(std::min<long long>(1 << 20, static_cast<long long>(q_len) * a.group));
+    return launch_any<false>(a, p, head_rows, head_dim, dtype, static_cast<hipStream_t>(stream));
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fa_attention_paged_workspace_bytes(int tokens, int num_seqs, int heads, int heads_kv, int head_dim,
+                                          int max_query_len, int max_kv_len)
+{
+    if (tokens <= 0 || num_seqs <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || head_dim <= 0 ||
+        max_query_len <= 0 || max_kv_len < 0)
+        return 0;
+    return make_plan(num_seqs, tokens, heads, heads_kv, head_dim, max_query_len, max_kv_len, true).workspace;
+}
+
+int fa_attention_paged_config(int tokens, int num_seqs, int heads, int heads_kv, int head_dim, int max_query_len,
+                              int max_kv_len, int* rows_per_block, int* splits)
+{
+    if (!rows_per_block || !splits) return fa::record_status(hipErrorInvalidValue);
+    *rows_per_block = *splits = 0;
+    if (head_dim != 64 && head_dim != 128) return FA_ERROR_UNSUPPORTED;
+    if (tokens <= 0 || num_seqs <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || max_query_len <= 0 ||
+        max_kv_len < 0)
+        return fa::record_status(hipErrorInvalidValue);
+    const Plan p = make_plan(num_seqs, tokens, heads, heads_kv, head_dim, max_query_len, max_kv_len, true);
+    *rows_per_block = 32 * p.waves;
+    *splits = p.splits;
+    return hipSuccess;
+}
+
+int fa_launch_attention_paged(const void* q, const fa_paged_cache* cache, void* o, void* workspace,
+                              size_t workspace_bytes, const int* block_table, const int* query_starts,
+                              const int* kv_lens, int num_seqs, int tokens, int heads, int table_width,
+                              long long table_stride, int max_query_len, int max_kv_len, int causal,
+                              const fa_strides* q_strides, const fa_strides* o_strides, void* stream)
+{
+    return fa::record_status(launch_paged(q, cache, o, workspace, workspace_bytes, block_table, table_stride, table_width,
+                                          query_starts, kv_lens, num_seqs, tokens, heads, max_query_len, max_kv_len, causal,
+                                          q_strides, o_strides, stream));
+}
+
+size_t fa_attention_cross_workspace_bytes(int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim)
+{
+    if (batch <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || q_len <= 0 || kv_len < 0 || head_dim <= 0)
+        return 0;
+    return make_plan(batch, static_cast<long long>(batch) * q_len, heads, heads_kv, head_dim, q_len, kv_len, false).workspace;
+}
+
+int fa_attention_cross_config(int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim,
+                              int* rows_per_block, int* splits)
+{
+    if (!rows_per_block || !splits) return fa::record_status(hipErrorInvalidValue);
+    *rows_per_block = *splits = 0;
+    if (head_dim != 64 && head_dim != 128) return FA_ERROR_UNSUPPORTED;
+    if (batch <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || q_len <= 0 || kv_len < 0)
+        return fa::record_status(hipErrorInvalidValue);
+    const Plan p = make_plan(batch, static_cast<long long>(batch) * q_len, heads, heads_kv, head_dim, q_len, kv_len, false);
+    *rows_per_block = 32 * p.waves;
+    *splits = p.splits;
+    return hipSuccess;
+}
+
+int fa_launch_attention_cross(const void* q, const void* k, const void* v, void* o, void* workspace,
+                              size_t workspace_bytes, const int* kv_lens, int batch, int heads, int heads_kv, int q_len,
+                              int kv_len, int head_dim, int dtype, const fa_strides* q_strides,
+                              const fa_strides* k_strides, const fa_strides* v_strides, const fa_strides* o_strides,
+                              void* stream)
+{
+    return fa::record_status(launch_cross(q, k, v, o, workspace, workspace_bytes, kv_lens, batch, heads, heads_kv, q_len,
+                                          kv_len, head_dim, dtype, q_strides, k_strides, v_strides, o_strides, stream));
+}
+
+}  // extern "C"

@@ -266,6 +266,121 @@ size_t fa_mfma_peak_records_bytes(void);
 int fa_mfma_peak(const void* operands, int mfma_per_wave, int launches, void* records, double* tflops,
                  double* clock_ghz, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Serving: attention of new tokens over a paged K/V cache, and of queries over
+ * an encoder's states of another length. No counterpart in the reference.
+ *
+ * Forward only, bf16 or fp16 (FA_DTYPE_*), fp32 accumulation, softmax scale
+ * 1/sqrt(head_dim); the heads of q that share a key head lie beside each other
+ * (query head h reads key head h / (heads / heads_kv)). Lengths, starts and
+ * block tables are device memory that the kernels read, so a captured launch
+ * follows them from replay to replay. The launchers allocate nothing and keep no
+ * state; a workspace belongs to one launch at a time, so launches that may
+ * overlap (other streams, replays of two graphs) need one each.
+ *
+ * Device pointers belong to the device that is current at the call, on whose
+ * stream the launch goes. A call returns as the launchers above do; refused on
+ * the host with hipErrorInvalidValue are also: bases off a 16-byte boundary,
+ * strides that are no multiple of 8 elements, key rows closer than head_dim or
+ * 2^26 elements or more apart, heads no multiple of heads_kv or above 65536,
+ * more than 2^30 keys of a sequence or rows (queries times heads per key head)
+ * of one, and a workspace that is missing or too small. */
+#define FA_DTYPE_BF16 0
+#define FA_DTYPE_FP16 1
+
+/* Distances in elements between batch entries, heads and rows; head_dim is
+ * contiguous. Where a pointer to these is NULL the tensor is contiguous. */
+typedef struct fa_strides {
+    long long batch;
+    long long head;
+    long long row;
+} fa_strides;
+
+/* A paged cache: num_blocks pages of block_size tokens (a power of two, 16 to
+ * 2^20) of heads_kv rows of head_dim elements. Token t of head h in page p is at
+ * p * block_stride + h * head_stride + t * token_stride (elements), in K as in V,
+ * so pages may hold [heads, tokens, dim] or [tokens, heads, dim]. Slot s is token
+ * s % block_size of page s / block_size. */
+typedef struct fa_paged_cache {
+    void* k;
+    void* v;
+    long long block_stride;
+    long long head_stride;
+    long long token_stride;
+    int num_blocks;
+    int heads_kv;
+    int block_size;
+    int head_dim;
+    int dtype;
+} fa_paged_cache;
+
+/* Block tables and slot maps from request lengths. Sequence s holds
+ * cached_lens[s] tokens and gets new_lens[s] more (negative counts are 0):
+ *   query_starts[num_seqs + 1]  where its new tokens start among all of them,
+ *                               and their number at the end;
+ *   kv_lens[num_seqs]           cached + new;
+ *   block_table                 [num_seqs, table_width] (rows table_stride apart):
+ *                               the entries of blocks that the new tokens open
+ *                               are taken from free_blocks[num_free], in order of
+ *                               the sequences, -1 where the list has ended; other
+ *                               entries stay;
+ *   slot_map[max_tokens]        each new token's slot; -1 where it has no block
+ *                               (the free list has ended, or the row's
+ *                               table_width * block_size is passed) and behind
+ *                               the last new token;
+ *   blocks_taken[1]             blocks opened; more than num_free: the list was
+ *                               too short.
+ * Tokens past max_tokens get no entry. All new tokens together: below 2^31. */
+int fa_launch_paged_slots(const int* cached_lens, const int* new_lens, int* block_table, const int* free_blocks,
+                          int* query_starts, int* kv_lens, long long* slot_map, int* blocks_taken, int num_seqs,
+                          int table_width, long long table_stride, int num_free, int block_size, int max_tokens,
+                          void* stream);
+
+/* Rows k, v [tokens, heads_kv, head_dim] (strides: row from token to token, head)
+ * into the slots slot_map names; a slot below 0 or past the cache is skipped.
+ * Slots are distinct (of two rows for one slot, either may be left, or pieces of
+ * both). Any head_dim that is a multiple of 8. */
+int fa_launch_paged_append(const void* k, const void* v, const long long* slot_map, const fa_paged_cache* cache,
+                           int tokens, const fa_strides* k_strides, const fa_strides* v_strides, void* stream);
+
+/* Attention of the new tokens q [tokens, heads, head_dim] over the cache, which
+ * holds their own keys already. Sequence s has the rows query_starts[s] ..
+ * query_starts[s + 1] - 1 of q; they are the last of its kv_lens[s] tokens.
+ * causal: a token sees the keys up to its own position; else all kv_lens[s]. A
+ * row that sees no key is 0. Rows of no sequence, and those past the first
+ * max_query_len of one, are left as they were. Keys past table_width *
+ * block_size do not exist; a table entry outside the cache stands for a page of
+ * zeros. What a page holds behind its sequence's length is never used. head_dim
+ * 64 or 128 (else FA_ERROR_UNSUPPORTED).
+ * max_query_len: no sequence has more new tokens. max_kv_len: about the most keys
+ * of one; it only decides how the work is split, any value gives the same
+ * result up to rounding. workspace: fa_attention_paged_workspace_bytes of the
+ * same numbers on the same device (0: may be NULL); fa_attention_paged_config:
+ * the rows of a workgroup and the most chunks a sequence's keys are split into. */
+size_t fa_attention_paged_workspace_bytes(int tokens, int num_seqs, int heads, int heads_kv, int head_dim,
+                                          int max_query_len, int max_kv_len);
+int fa_attention_paged_config(int tokens, int num_seqs, int heads, int heads_kv, int head_dim, int max_query_len,
+                              int max_kv_len, int* rows_per_block, int* splits);
+int fa_launch_attention_paged(const void* q, const fa_paged_cache* cache, void* o, void* workspace,
+                              size_t workspace_bytes, const int* block_table, const int* query_starts,
+                              const int* kv_lens, int num_seqs, int tokens, int heads, int table_width,
+                              long long table_stride, int max_query_len, int max_kv_len, int causal,
+                              const fa_strides* q_strides, const fa_strides* o_strides, void* stream);
+
+/* Attention of q [batch, heads, q_len, head_dim] to an encoder's states k, v
+ * [batch, heads_kv, kv_len, head_dim]: every query of entry b sees its first
+ * kv_lens[b] states (NULL: all kv_len; values are clamped to 0 .. kv_len), and
+ * what lies behind them is never used. With no state a row is 0. head_dim 64 or
+ * 128 (else FA_ERROR_UNSUPPORTED). The workspace and the config: as above. */
+size_t fa_attention_cross_workspace_bytes(int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim);
+int fa_attention_cross_config(int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim,
+                              int* rows_per_block, int* splits);
+int fa_launch_attention_cross(const void* q, const void* k, const void* v, void* o, void* workspace,
+                              size_t workspace_bytes, const int* kv_lens, int batch, int heads, int heads_kv, int q_len,
+                              int kv_len, int head_dim, int dtype, const fa_strides* q_strides,
+                              const fa_strides* k_strides, const fa_strides* v_strides, const fa_strides* o_strides,
+                              void* stream);
+
 /* Library identification: "gfx950" and the build's kernel configuration. */
 const char* fa_build_info(void);
 

@@ -1,0 +1,525 @@
+"""Serving operators on the GPU against plain forms in 64 bits (serving_ref.py),
+at the lengths, masks, layouts and pages where they can go wrong."""
+import math
+
+import pytest
+import torch
+
+import serving_ref as ref
+from gpu_common import say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def fa(fa_lib):
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a visible MI355X")
+    return fa_lib
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(shape, dtype, g, scale=1.0):
+    return (torch.randn(shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def heads_view(x, layout):
+    return x if layout == "HND" else x.transpose(1, 2).contiguous().transpose(1, 2)
+
+
+def ints(x, dtype=torch.int32):
+    return torch.tensor(x, dtype=dtype, device="cuda")
+
+
+class Paged:
+    """A batch over a cache whose unused slots hold NaN."""
+
+    def __init__(self, fa, cached, new, heads, heads_kv, dim, block, dtype, layout="HND", seed=1, extra_rows=0,
+                 extra_width=0, scale=1.0, fill=float("nan")):
+        g = gen(seed)
+        self.kv = [c + n for c, n in zip(cached, new)]
+        need = [-(-x // block) for x in self.kv]
+        blocks = sum(need) + 3
+        self.block, self.dtype = block, ref.TYPES[dtype]
+        shape = (blocks, heads_kv, block, dim)
+        self.k, self.v = (heads_view(torch.full(shape, fill, device="cuda", dtype=self.dtype), layout) for _ in range(2))
+        order = torch.randperm(blocks, device="cuda", generator=g).tolist()
+        width = max(max(need, default=0), 1) + extra_width
+        table = [[-7] * width for _ in need]
+        at = 0
+        for s, n in enumerate(need):
+            for b in range(n):
+                table[s][b] = order[at]
+                count = min(block, self.kv[s] - b * block)
+                self.k[order[at], :, :count] = randn((heads_kv, count, dim), self.dtype, g, scale)
+                self.v[order[at], :, :count] = randn((heads_kv, count, dim), self.dtype, g)
+                at += 1
+        self.table = ints(table).reshape(len(need), width)
+        self.starts = [0]
+        for n in new:
+            self.starts.append(self.starts[-1] + n)
+        self.q = randn((self.starts[-1] + extra_rows, heads, dim), self.dtype, g, scale)
+        self.max_new = max(new, default=0)
+        self.cache = fa.paged_cache(self.k, self.v)
+
+    def run(self, fa, causal=True, out=None, max_kv_len=None, **more):
+        if out is None:
+            out = torch.full_like(self.q, float("nan"))
+        fa.attention_paged(self.q, self.cache, self.table, ints(self.starts), ints(self.kv), self.max_new, max_kv_len,
+                           causal=causal, out=out, **more)
+        torch.cuda.synchronize()
+        return out
+
+    def check(self, fa, causal=True, what="", **more):
+        got = self.run(fa, causal, **more)
+        want, tol, inside = ref.paged(self.q, self.k, self.v, self.table, self.starts, self.kv, self.block, causal)
+        ref.check(got[inside], want[inside], tol[inside], what)
+        assert got[~inside].isnan().all(), "rows of no sequence were written"
+        return got
+
+
+# ---------------------------------------------------------------- block tables and slots
+@pytest.mark.parametrize("cached,new,block", [
+    ([0], [1], 16), ([15], [1], 16), ([16], [1], 16), ([17], [40], 16), ([0], [0], 16), ([5], [0], 32),
+    ([0, 0, 7, 31, 32, 33, 64], [0, 5, 0, 1, 1, 100, 0], 32),
+    ([100] * 64, [1] * 64, 128),
+])
+def test_slots_small(fa, cached, new, block):
+    say("slots", cached, new, block)
+    _check_slots(fa, cached, new, block)
+
+
+def _check_slots(fa, cached, new, block, free_cut=0, width_cut=0, pad=5, row_gap=0, out=None, token_cut=0):
+    cached_p, new_p = [max(c, 0) for c in cached], [max(n, 0) for n in new]
+    have = [-(-c // block) for c in cached_p]
+    need = [-(-(c + n) // block) for c, n in zip(cached_p, new_p)]
+    width = max(max(need, default=1), 1) - width_cut
+    pages = torch.randperm(sum(need) + 9, generator=torch.Generator().manual_seed(3)).tolist()
+    table = [[-5] * width for _ in cached]
+    at = 0
+    for s, n in enumerate(have):
+        for b in range(min(n, width)):
+            table[s][b] = pages[at]
+            at += 1
+    free = pages[at:at + max(0, sum(need) - sum(have) - free_cut)]
+    tokens = max(0, sum(new_p) + pad - token_cut)
+    want = ref.slots(cached, new, table, free, block, tokens)
+    wide = torch.full((len(cached), width + row_gap), -9, dtype=torch.int32, device="cuda")
+    dev = wide[:, :width]
+    if cached:
+        dev.copy_(ints(table))
+    got = fa.paged_slots(ints(cached), ints(new), dev, ints(free), block, tokens, out=out)
+    torch.cuda.synchronize()
+    assert dev.tolist() == want[0]
+    assert (wide[:, width:] == -9).all()
+    assert got.query_starts.tolist() == want[1] and got.kv_lens.tolist() == want[2]
+    assert got.slot_map.tolist() == want[3] and got.blocks_taken.tolist() == [want[4]]
+
+
+@pytest.mark.parametrize("seqs,block,seed", [(1, 16, 1), (63, 16, 2), (64, 32, 3), (65, 16, 4), (255, 16, 5), (256, 64, 6),
+                                              (257, 16, 7), (1023, 16, 8), (1025, 32, 9), (2500, 16, 10)])
+def test_slots_many(fa, seqs, block, seed):
+    import random
+
+    rng = random.Random(seed)
+    cached = [rng.choice([0, rng.randint(0, 300)]) for _ in range(seqs)]
+    new = [rng.choice([0, 1, 1, 1, rng.randint(0, 90)]) for _ in range(seqs)]
+    say("slots", seqs, block, seed)
+    _check_slots(fa, cached, new, block)
+    _check_slots(fa, cached, new, block, row_gap=3, token_cut=min(40, sum(new)), pad=0)
+
+
+def test_slots_ends(fa):
+    """A short free list, a narrow table, negative lengths, no sequence, one long prompt."""
+    cached, new = [3, 40, 0, 16], [20, 33, 64, 1]
+    for cut in (1, 3, 100):
+        say("slots free cut", cut)
+        _check_slots(fa, cached, new, 16, free_cut=cut)
+    for cut in (1, 2, 3):
+        say("slots width cut", cut)
+        _check_slots(fa, cached, new, 16, width_cut=cut)
+    _check_slots(fa, [-3, 5, -1], [4, -9, -2], 16)
+    _check_slots(fa, [], [], 16)
+    _check_slots(fa, [7], [70000], 16)
+    _check_slots(fa, [0] * 300, [200] * 300, 64, pad=0)
+
+
+# ---------------------------------------------------------------- cache writes
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+@pytest.mark.parametrize("tokens,heads_kv,dim,block", [(1, 1, 64, 16), (7, 8, 128, 16), (129, 5, 64, 32), (33, 2, 8, 16),
+                                                       (1000, 4, 96, 128), (3, 16, 128, 1024)])
+def test_append(fa, dtype, layout, tokens, heads_kv, dim, block):
+    say("append", dtype, layout, tokens, heads_kv, dim, block)
+    g, t = gen(tokens), ref.TYPES[dtype]
+    blocks = -(-tokens // block) + 2
+    k, v = (heads_view(randn((blocks, heads_kv, block, dim), t, g), layout) for _ in range(2))
+    slots = torch.randperm(blocks * block, device="cuda", generator=g)[:tokens].contiguous()
+    slots[tokens // 2] = -1
+    if tokens > 4:
+        slots[0], slots[4] = blocks * block, -(2 ** 62)
+        slots[1] = 2 ** 62
+    qkv = randn((tokens, heads_kv + 2 * heads_kv, dim), t, g)
+    new_k, new_v = qkv[:, heads_kv:2 * heads_kv], qkv[:, 2 * heads_kv:]
+    want_k, want_v = k.clone(), v.clone()
+    for i, s in enumerate(slots.tolist()):
+        if 0 <= s < blocks * block:
+            want_k[s // block, :, s % block] = new_k[i]
+            want_v[s // block, :, s % block] = new_v[i]
+    fa.paged_append(new_k, new_v, slots, fa.paged_cache(k, v))
+    torch.cuda.synchronize()
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+    fa.paged_append(new_k[:0], new_v[:0], slots[:0], fa.paged_cache(k, v))
+    torch.cuda.synchronize()
+    assert torch.equal(k, want_k)
+
+
+# ---------------------------------------------------------------- attention over the cache
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,heads_kv", [(1, 1), (8, 8), (8, 2), (7, 1), (12, 4)])
+def test_paged_decode(fa, dtype, dim, heads, heads_kv):
+    cached = [0, 1, 14, 15, 16, 30, 31, 32, 33, 63, 64, 65, 200, 511]
+    for layout, block in (("HND", 16), ("NHD", 32), ("HND", 128)):
+        say("decode", dtype, dim, heads, heads_kv, layout, block)
+        Paged(fa, cached, [1] * len(cached), heads, heads_kv, dim, block, dtype, layout, seed=block).check(fa, what="decode")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_paged_chunks(fa, dtype, dim, causal):
+    """Chunks of every size class of the row blocks, beside decoding sequences."""
+    for cached, new, heads, heads_kv in (
+            ([0, 3, 100], [1, 2, 3], 4, 2), ([70, 0, 33, 5], [33, 64, 1, 9], 1, 1), ([0, 500, 17], [130, 65, 127], 4, 4),
+            ([200, 1, 0, 31], [257, 1, 300, 16], 6, 2), ([0], [1100], 2, 1), ([900, 4], [40, 1], 16, 1)):
+        for layout, block in (("HND", 16), ("NHD", 64)):
+            say("chunks", dtype, dim, causal, cached, new, heads, heads_kv, layout, block)
+            Paged(fa, cached, new, heads, heads_kv, dim, block, dtype, layout, seed=len(cached),
+                  extra_rows=3).check(fa, causal, "chunks")
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("fp16", 64), ("bf16", 64), ("fp16", 128)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_paged_splits(fa, dtype, dim, causal):
+    """Long caches, whose keys are split over workgroups and joined; short ones beside
+    them, and a hint that is far off."""
+    for cached, new, heads, heads_kv in (([4000], [1], 4, 2), ([3000, 0, 257, 512, 2047], [1, 1, 1, 1, 1], 8, 1),
+                                         ([2500, 100], [70, 40], 2, 1), ([5000], [300], 1, 1), ([2222, 0], [9, 9], 4, 1)):
+        b = Paged(fa, cached, new, heads, heads_kv, dim, 16, dtype, seed=7, extra_rows=2)
+        rows, splits = fa.attention_paged_config(b.q.shape[0], len(new), heads, heads_kv, dim, b.max_new, max(b.kv))
+        say("splits", dtype, dim, causal, cached, new, rows, splits)
+        assert splits > 1
+        b.check(fa, causal, "splits")
+        b.check(fa, causal, "splits, long hint", max_kv_len=100000)
+        b.check(fa, causal, "splits, short hint", max_kv_len=600)
+        b.check(fa, causal, "splits, no hint", max_kv_len=0)
+
+
+def test_paged_empty_rows(fa):
+    """No keys, more new tokens than keys, no new tokens, no sequences."""
+    b = Paged(fa, [0, 5, 0, 40], [0, 3, 70, 1], 4, 2, 64, 16, "bf16", extra_rows=4)
+    b.kv[1], b.kv[2], b.kv[3] = 0, 50, -3  # lengths below the new tokens': the first rows see nothing
+    say("empty rows")
+    got = b.check(fa, True, "empty")
+    assert (got[:3] == 0).all() and (got[3:23] == 0).all() and (got[73] == 0).all()
+    b.check(fa, False, "empty, all keys")
+    out = torch.full_like(b.q, 7.0)
+    fa.attention_paged(b.q, b.cache, b.table[:0], ints([0]), ints([]), 1, out=out)
+    fa.attention_paged(b.q[:0], b.cache, b.table, ints([0] * 5), ints(b.kv), 1, out=out[:0])
+    fa.attention_paged(b.q, b.cache, b.table, ints(b.starts), ints(b.kv), 0, out=out)
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+
+
+def test_paged_pages_outside_the_cache(fa):
+    """A page that does not exist holds zeros; keys past the table do not exist."""
+    for dim, cached, new in ((64, [40, 700], [1, 3]), (128, [33, 100], [200, 17])):
+        b = Paged(fa, cached, new, 4, 2, dim, 16, "bf16", seed=5)
+        b.table[0, 1] = -1
+        b.table[1, 0] = b.cache.num_blocks
+        b.table[1, 3] = 2 ** 31 - 1
+        b.table[1, 4] = -2 ** 31
+        say("pages", dim)
+        b.check(fa, True, "pages")
+        b.table = b.table[:, :5]
+        b.check(fa, True, "narrow table")
+        b.check(fa, False, "narrow table, all keys")
+    b.table = b.table[:, :0]
+    got = b.run(fa)
+    assert (got == 0).all()
+
+
+def test_paged_rows_past_max_query_len(fa):
+    b = Paged(fa, [10, 20], [9, 4], 4, 2, 64, 16, "bf16")
+    for limit in (4, 6, 100):
+        b.max_new = limit
+        say("max_query_len", limit)
+        got = b.run(fa)
+        want, tol, _ = ref.paged(b.q, b.k, b.v, b.table, b.starts, b.kv, 16, True)
+        n = min(limit, 9)
+        ref.check(got[:n], want[:n], tol[:n], "first rows")
+        ref.check(got[9:], want[9:], tol[9:], "second sequence")
+        assert got[n:9].isnan().all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_paged_many_sequences(fa, causal):
+    """Row blocks that are found among many sequences, some of them without new tokens."""
+    import random
+
+    rng = random.Random(4)
+    for seqs, top in ((70, 150), (300, 90)):
+        new = [rng.choice([0, 1, 1, 2, rng.randint(0, 5)]) for _ in range(seqs)]
+        for s in rng.sample(range(seqs), 5):
+            new[s] = rng.randint(40, top)
+        cached = [rng.randint(0, 50) for _ in range(seqs)]
+        say("many", seqs, causal)
+        Paged(fa, cached, new, 4, 1, 64, 16, "bf16", seed=seqs, extra_rows=7).check(fa, causal, "many sequences")
+
+
+def test_paged_views(fa):
+    """Strided q and out, a wide table's columns, a cache between other data."""
+    b = Paged(fa, [30, 0, 77], [5, 40, 1], 4, 2, 64, 16, "bf16", "NHD", extra_rows=1)
+    qkv = torch.zeros((b.q.shape[0], 9, 64), dtype=b.dtype, device="cuda")
+    qkv[:, 2:6] = b.q
+    b.q = qkv[:, 2:6]
+    wide = torch.full((3, b.table.shape[1] + 5), -3, dtype=torch.int32, device="cuda")
+    wide[:, :b.table.shape[1]] = b.table
+    b.table = wide[:, :b.table.shape[1]]
+    both = torch.full((b.k.shape[0], 3, 16, 2, 64), float("nan"), dtype=b.dtype, device="cuda")
+    both[:, 0], both[:, 2] = b.k.transpose(1, 2), b.v.transpose(1, 2)
+    b.cache = fa.paged_cache(both[:, 0].transpose(1, 2), both[:, 2].transpose(1, 2))
+    room = torch.full((b.q.shape[0], 6, 64), float("nan"), dtype=b.dtype, device="cuda")
+    say("views")
+    b.check(fa, True, "views", out=room[:, 1:5])
+    assert room[:, 0].isnan().all() and room[:, 5].isnan().all()
+
+
+def test_paged_past_32_bits(fa):
+    """Pages whose bytes lie past 2^32, and a page and a head stride that span it."""
+    dim, block, heads_kv = 128, 16, 2
+    room = torch.zeros(3 * 2 ** 30, dtype=torch.bfloat16, device="cuda")  # 6 GiB
+    g = gen(2)
+    page = 1 << 28  # elements from page to page
+    shape, strides = (10, heads_kv, block, dim), (page, 1 << 27, dim, 1)
+    k = room.as_strided(shape, strides)
+    v = room[1 << 20:].as_strided(shape, strides)
+    for c in (k, v):
+        c.copy_(randn(shape, torch.bfloat16, g))
+    table = ints([[9, 0, 8, 3, 7], [1, 9, 2, 8, 5]])
+    starts, kv = [0, 1, 40], [70, 79]
+    q = randn((40, 4, dim), torch.bfloat16, g)
+    say("past 32 bits")
+    got = fa.attention_paged(q, fa.paged_cache(k, v), table, ints(starts), ints(kv), 39)
+    torch.cuda.synchronize()
+    want, tol, _ = ref.paged(q, k, v, table, starts, kv, block, True)
+    ref.check(got, want, tol, "past 32 bits")
+    slots = ints([9 * 16 + 3, 8 * 16 + 15], torch.int64)
+    rows = randn((2, heads_kv, dim), torch.bfloat16, g)
+    fa.paged_append(rows, rows, slots, fa.paged_cache(k, v))
+    torch.cuda.synchronize()
+    assert torch.equal(k[9, :, 3], rows[0]) and torch.equal(v[8, :, 15], rows[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_paged_large_scores(fa, dtype):
+    """Scores whose maximum keeps growing along a row, and far apart."""
+    b = Paged(fa, [1500, 60], [3, 50], 4, 2, 64, 16, dtype, seed=11, scale=4.0)
+    say("large scores", dtype)
+    b.check(fa, True, "large scores")
+
+
+# ---------------------------------------------------------------- attention to an encoder's states
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len,kv_len", [(1, 1), (1, 700), (3, 31), (17, 32), (33, 33), (64, 65), (100, 1), (129, 257),
+                                          (300, 95), (1, 3001), (40, 2048)])
+def test_cross(fa, dtype, dim, q_len, kv_len):
+    for batch, heads, heads_kv, layout, padded in ((1, 1, 1, "HND", False), (3, 6, 2, "NHD", True), (2, 5, 5, "HND", True)):
+        say("cross", dtype, dim, q_len, kv_len, batch, heads, heads_kv, layout, padded)
+        g, t = gen(q_len * 7 + kv_len), ref.TYPES[dtype]
+        q = heads_view(randn((batch, heads, q_len, dim), t, g), layout)
+        k, v = (heads_view(randn((batch, heads_kv, kv_len, dim), t, g), layout) for _ in range(2))
+        lens = [kv_len] * batch
+        if padded:
+            lens = [kv_len, max(0, kv_len - 5), 0, 1][:batch]
+            for b, m in enumerate(lens):  # the padding is never used
+                k[b, :, m:], v[b, :, m:] = float("nan"), float("inf")
+        out = torch.full_like(q, float("nan"))
+        fa.attention_cross(q, k, v, ints(lens) if padded else None, out=out)
+        torch.cuda.synchronize()
+        want, tol = ref.cross(q, k, v, lens)
+        ref.check(out, want, tol, "cross")
+
+
+def test_cross_ends(fa):
+    """No states, lengths out of range, nothing to do, shared states (stride 0)."""
+    g = gen(1)
+    q = randn((3, 4, 9, 64), torch.bfloat16, g)
+    k, v = (randn((1, 2, 50, 64), torch.bfloat16, g) for _ in range(2))
+    ke, ve = k.expand(3, 2, 50, 64), v.expand(3, 2, 50, 64)
+    say("cross ends")
+    got = fa.attention_cross(q, ke, ve, ints([-4, 50, 1000]))
+    torch.cuda.synchronize()
+    want, tol = ref.cross(q, ke, ve, [0, 50, 50])
+    ref.check(got, want, tol, "lengths")
+    none = fa.attention_cross(q, ke[:, :, :0], ve[:, :, :0])
+    torch.cuda.synchronize()
+    assert (none == 0).all()
+    assert fa.attention_cross(q[:0], ke[:0], ve[:0]).shape[0] == 0
+    assert fa.attention_cross(q[:, :, :0], ke, ve).shape[2] == 0
+
+
+def test_cross_is_the_self_attention(fa):
+    """With as many keys as queries: the fused forward's result, each within its rounding."""
+    g = gen(8)
+    q, k, v = (randn((2, 4, 384, 128), torch.bfloat16, g) for _ in range(3))
+    say("cross as self")
+    got = fa.attention_cross(q, k, v)
+    base = fa.attention_forward(q, k, v)
+    torch.cuda.synchronize()
+    _, tol = ref.cross(q, k, v, [384, 384])
+    ref.check(got, base.double(), 2 * tol, "self")
+
+
+# ---------------------------------------------------------------- how they are called
+def _serve(fa, layout, dtype, steps, graph):
+    """A prompt in chunks, then decoding, each step: slots, writes, attention."""
+    dim, heads, heads_kv, block, seqs, t = 64, 4, 2, 16, 3, ref.TYPES[dtype]
+    g = gen(3)
+    k, v = (heads_view(torch.full((40, heads_kv, block, dim), float("nan"), device="cuda", dtype=t), layout) for _ in range(2))
+    cache = fa.paged_cache(k, v)
+    table = torch.full((seqs, 12), -1, dtype=torch.int32, device="cuda")
+    pages = torch.randperm(40, device="cuda", generator=g).to(torch.int32)
+    cached, new = torch.zeros(seqs, dtype=torch.int32, device="cuda"), torch.zeros(seqs, dtype=torch.int32, device="cuda")
+    free = pages.clone()
+    rows = 64
+    q, nk, nv = (torch.zeros((rows, n, dim), device="cuda", dtype=t) for n in (heads, heads_kv, heads_kv))
+    bufs = fa.paged_slots_buffers(seqs, rows)
+    out = torch.empty_like(q)
+    ws = fa.attention_paged_workspace(q, cache, seqs, 50, 12 * block)
+
+    def step():
+        fa.paged_slots(cached, new, table, free, block, rows, out=bufs)
+        fa.paged_append(nk, nv, bufs.slot_map, cache)
+        fa.attention_paged(q, cache, table, bufs.query_starts, bufs.kv_lens, 50, out=out, workspace=ws)
+
+    captured = None
+    if graph:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        captured = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(captured):
+            step()
+    results, taken = [], 0
+    history = [[torch.zeros((0, heads_kv, dim), dtype=t, device="cuda")] * 2 for _ in range(seqs)]
+    lens = [0] * seqs
+    for counts in steps:
+        cached.copy_(ints(lens))
+        new.copy_(ints(counts))
+        free.copy_(torch.roll(pages, -taken))
+        for x in (q, nk, nv):
+            x.copy_(randn(x.shape, t, g))
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        captured.replay() if graph else step()
+        torch.cuda.synchronize()
+        taken += int(bufs.blocks_taken)
+        at = 0
+        for s, n in enumerate(counts):
+            history[s] = [torch.cat([history[s][0], nk[at:at + n]]), torch.cat([history[s][1], nv[at:at + n]])]
+            for h in range(heads):
+                limits = lens[s] + 1 + torch.arange(n, device="cuda")
+                want, tol = ref.attend(q[at:at + n, h], history[s][0][:, h // 2], history[s][1][:, h // 2], limits)
+                ref.check(out[at:at + n, h], want, tol, f"step {counts} sequence {s}")
+            lens[s] += n
+            at += n
+        assert out[at:].isnan().all()
+        results.append(out.clone())
+    return results
+
+
+STEPS = [[40, 1, 0], [1, 17, 0], [1, 1, 50], [1, 1, 1], [0, 1, 1], [1, 0, 30], [1, 1, 1]]
+
+
+@pytest.mark.parametrize("layout,dtype", [("HND", "bf16"), ("NHD", "fp16")])
+def test_serving_run(fa, layout, dtype):
+    say("serving run", layout, dtype)
+    eager = _serve(fa, layout, dtype, STEPS, False)
+    say("serving run captured", layout, dtype)
+    replayed = _serve(fa, layout, dtype, STEPS, True)
+    for a, b in zip(eager, replayed):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def test_streams_and_repeats(fa):
+    """On another stream than the current one, and bitwise the same every time, with a
+    split launch's workspace full of NaN at the start."""
+    b = Paged(fa, [3000, 20], [1, 30], 4, 1, 128, 16, "bf16", seed=9)
+    ws = fa.attention_paged_workspace(b.q, b.cache, 2, b.max_new, max(b.kv))
+    assert ws is not None
+    ws.fill_(255)
+    first = b.run(fa, workspace=ws, max_kv_len=max(b.kv))
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = b.run(fa, workspace=ws, max_kv_len=max(b.kv))
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(first.view(torch.int16), again.view(torch.int16))
+    say("streams")
+
+
+def test_refusals(fa):
+    b = Paged(fa, [10], [2], 4, 2, 64, 16, "bf16")
+    starts, kv = ints(b.starts), ints(b.kv)
+
+    def call(q=b.q, cache=b.cache, table=b.table, starts=starts, kv=kv, n=2, **more):
+        return fa.attention_paged(q, cache, table, starts, kv, n, **more)
+
+    for bad in (dict(q=b.q.half()), dict(q=b.q[:, :, :32]), dict(q=b.q.cpu()), dict(table=b.table.long()),
+                dict(starts=starts[:1]), dict(kv=kv.long()), dict(out=b.q.half()), dict(table=b.table[:0]),
+                dict(q=b.q.transpose(1, 2).contiguous().transpose(1, 2))):
+        with pytest.raises(ValueError):
+            call(**bad)
+    with pytest.raises(fa.FaError):
+        call(q=randn((2, 3, 64), torch.bfloat16, gen(1)))  # heads no multiple of the key heads
+    with pytest.raises(fa.FaError):
+        call(n=-1)
+    long = Paged(fa, [5000], [1], 4, 2, 64, 16, "bf16")
+    with pytest.raises(ValueError):
+        fa.attention_paged(long.q, long.cache, long.table, ints(long.starts), ints(long.kv), 1,
+                           workspace=torch.empty(8, dtype=torch.uint8, device="cuda"))
+    odd = torch.zeros((4, 2, 16, 96), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        fa.attention_paged(torch.zeros((1, 2, 96), dtype=torch.bfloat16, device="cuda"), fa.paged_cache(odd, odd),
+                           ints([[0]]), ints([0, 1]), ints([1]), 1)
+    with pytest.raises(ValueError):
+        fa.paged_cache(b.k, b.v.transpose(1, 2).contiguous().transpose(1, 2) if b.k.is_contiguous() else b.v.contiguous())
+    with pytest.raises(ValueError):
+        fa.paged_cache(b.k.float(), b.v.float())
+    q, k = torch.zeros((1, 4, 3, 64), device="cuda"), torch.zeros((1, 2, 5, 64), device="cuda")
+    with pytest.raises(ValueError):
+        fa.attention_cross(q, k, k)
+    q, k = q.bfloat16(), k.bfloat16()
+    with pytest.raises(ValueError):
+        fa.attention_cross(q, k.half(), k.half())
+    with pytest.raises(ValueError):
+        fa.attention_cross(q, k, k, ints([5, 5]))
+    with pytest.raises(fa.FaError):
+        fa.attention_cross(q, k[:, :, :1].expand(1, 2, 5, 64), k)  # key rows on top of each other
+    with pytest.raises(ValueError):
+        fa.paged_slots(ints([1]), ints([1, 2]), ints([[0]]), ints([1]), 16, 4)
+    with pytest.raises(fa.FaError):
+        fa.paged_slots(ints([1]), ints([1]), ints([[0]]), ints([1]), 24, 4)
+    with pytest.raises(ValueError):
+        fa.paged_append(q[0], q[0], ints([0, 1, 2, 3]), b.cache)
+    torch.cuda.synchronize()
