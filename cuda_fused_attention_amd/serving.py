@@ -13,7 +13,6 @@ run on the current stream of the tensors' device. Forward only.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import NamedTuple, Optional
 
@@ -121,23 +120,35 @@ def launch_attention_cross(q, k, v, o, workspace, workspace_bytes: int, kv_lens,
 
 
 # ---------------------------------------------------------------- torch convenience
+# torch, the element types and the current device, bound on first use (torch is
+# imported only for torch callers). These functions are on the path of every
+# decoding step, so a check costs its comparisons and builds no message.
+_torch = None
+_dtype_ids = {}
+_current_device = None
+
+
+def _bind():
+    global _torch, _dtype_ids, _current_device
+    import torch
+
+    _dtype_ids = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16}
+    _current_device = torch.cuda.current_device
+    _torch = torch
+    return torch
+
+
 def _dtype_id(dtype) -> int:
-    import torch
-
-    if dtype == torch.bfloat16:
-        return DTYPE_BF16
-    if dtype == torch.float16:
-        return DTYPE_FP16
-    raise ValueError(f"bf16 or fp16 tensors are needed, not {dtype}")
+    if dtype not in _dtype_ids:
+        raise ValueError(f"bf16 or fp16 tensors are needed, not {dtype}")
+    return _dtype_ids[dtype]
 
 
-def _on(device):
-    """The context in which `device` is the current one."""
-    import torch
-
+def _elsewhere(device) -> bool:
+    """Whether `device` is another GPU than the current one."""
     if device.type != "cuda":
         raise ValueError("CUDA tensors are needed")
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return device.index != _current_device()
 
 
 def _need(ok: bool, what: str):
@@ -145,43 +156,53 @@ def _need(ok: bool, what: str):
         raise ValueError(what)
 
 
-def _int32(x, name: str, shape, device):
-    """`x` is a contiguous int32 tensor of this shape on this device."""
-    import torch
-
-    _need(x.dtype == torch.int32 and x.device == device and tuple(x.shape) == shape and x.is_contiguous(),
-          f"{name} must be a contiguous int32 tensor {list(shape)} on {device}")
+def _vector(x, n: int, device, dtype, name: str):
+    """`x` is a contiguous vector of n integers on this device."""
+    if x.dtype != dtype or x.device != device or tuple(x.shape) != (n,) or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor [{n}] on {device}")
 
 
-def _table(block_table, num_seqs, device):
+def _table(table, num_seqs: int, device):
     """(width, row stride) of a block table."""
-    import torch
-
-    _need(block_table.dtype == torch.int32 and block_table.device == device and block_table.dim() == 2
-          and block_table.shape[0] == num_seqs, f"block_table must be an int32 tensor [{num_seqs}, width] on {device}")
-    width = block_table.shape[1]
-    stride = block_table.stride(0) if num_seqs > 1 else max(width, 1)
-    _need(width <= 1 or block_table.stride(1) == 1, "block_table rows must be contiguous")
-    _need(stride >= width, "block_table rows must not overlap")
+    if table.dtype != _torch.int32 or table.device != device or table.dim() != 2 or table.shape[0] != num_seqs:
+        raise ValueError(f"block_table must be an int32 tensor [{num_seqs}, width] on {device}")
+    width = table.shape[1]
+    stride, column = table.stride()
+    if num_seqs < 2:
+        stride = max(width, 1)
+    if (width > 1 and column != 1) or stride < width:
+        raise ValueError("block_table: entries of a row must be contiguous, rows must not overlap")
     return width, stride
 
 
-def _stride(x, dim: int) -> int:
-    """The distance along `dim`; where it has one entry, whose stride means nothing,
-    one row."""
-    return x.stride(dim) if x.shape[dim] > 1 else x.shape[-1]
+def _strides_of(x, name: str):
+    """Strides (batch, head, row) of a [batch, heads, rows, dim] tensor, (0, head, row)
+    of a [rows, heads, dim] one. Along an axis of one entry, whose stride means
+    nothing, one row."""
+    shape, stride = x.shape, x.stride()
+    dim = shape[-1]
+    if stride[-1] != 1:
+        raise ValueError(f"{name}: head_dim must be contiguous")
+    if len(shape) == 3:
+        return 0, stride[1] if shape[1] > 1 else dim, stride[0] if shape[0] > 1 else dim
+    return (stride[0] if shape[0] > 1 else dim, stride[1] if shape[1] > 1 else dim, stride[2] if shape[2] > 1 else dim)
 
 
-def _row_strides(x, name: str):
-    """Strides (0, head, row) of a [rows, heads, dim] tensor."""
-    _need(x.stride(2) == 1, f"{name}: head_dim must be contiguous")
-    return 0, _stride(x, 1), _stride(x, 0)
+def _like_q(out, q):
+    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must have q's shape, type and device")
 
 
-def _head_strides(x, name: str):
-    """Strides (batch, head, row) of a [batch, heads, rows, dim] tensor."""
-    _need(x.stride(3) == 1, f"{name}: head_dim must be contiguous")
-    return _stride(x, 0), _stride(x, 1), _stride(x, 2)
+def _workspace_room(workspace, device) -> int:
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    return workspace.numel() * workspace.element_size()
+
+
+def _too_small(workspace, have: int, nbytes: int):
+    """Says so where a refused launch's workspace was too small."""
+    if workspace is not None and have < nbytes:
+        raise ValueError(f"workspace holds {have} bytes, {nbytes} are needed")
 
 
 def paged_cache(k_cache, v_cache) -> PagedCache:
@@ -189,14 +210,14 @@ def paged_cache(k_cache, v_cache) -> PagedCache:
     fp16, equal strides, head_dim contiguous). Pages that hold their tokens' heads
     side by side, [num_blocks, block_size, heads_kv, head_dim], come as
     .transpose(1, 2)."""
+    if _torch is None:
+        _bind()
     _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "k_cache, v_cache: [num_blocks, heads_kv, block_size, head_dim]")
     _need(k_cache.dtype == v_cache.dtype and k_cache.device == v_cache.device, "k_cache and v_cache differ in type or device")
     _need(k_cache.is_cuda, "CUDA tensors are needed")
-    _need(k_cache.stride(3) == 1 and v_cache.stride(3) == 1
-          and all(_stride(k_cache, d) == _stride(v_cache, d) for d in range(3)),
-          "k_cache and v_cache must have equal strides, head_dim contiguous")
+    block, head, token = _strides_of(k_cache, "k_cache")
+    _need((block, head, token) == _strides_of(v_cache, "v_cache"), "k_cache and v_cache must have equal strides")
     num_blocks, heads_kv, block_size, head_dim = k_cache.shape
-    block, head, token = (_stride(k_cache, d) for d in range(3))
     info = _fa.PagedCacheInfo(k_cache.data_ptr(), v_cache.data_ptr(), block, head, token, num_blocks, heads_kv, block_size,
                               head_dim, _dtype_id(k_cache.dtype))
     return PagedCache(k_cache, v_cache, info)
@@ -204,7 +225,7 @@ def paged_cache(k_cache, v_cache) -> PagedCache:
 
 def paged_slots_buffers(num_seqs: int, max_tokens: int, device="cuda") -> PagedSlots:
     """Buffers that paged_slots can write again and again (`out`)."""
-    import torch
+    torch = _torch or _bind()
 
     def ints(n, dtype=torch.int32):
         return torch.empty(n, dtype=dtype, device=device)
@@ -219,66 +240,51 @@ def paged_slots(cached_lens, new_lens, block_table, free_blocks, block_size: int
     [num_seqs, width] for the blocks that the new tokens open are taken from
     free_blocks, in order; every new token gets its slot in slot_map (-1: none).
     All int32; what happens at the ends is written at fa_launch_paged_slots."""
-    import torch
-
+    torch = _torch or _bind()
     device = cached_lens.device
-    _need(cached_lens.dim() == 1 and free_blocks.dim() == 1, "cached_lens and free_blocks must be vectors")
-    num_seqs = cached_lens.shape[0]
-    _int32(cached_lens, "cached_lens", (num_seqs,), device)
-    _int32(new_lens, "new_lens", (num_seqs,), device)
-    _int32(free_blocks, "free_blocks", (free_blocks.shape[0],), device)
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return paged_slots(cached_lens, new_lens, block_table, free_blocks, block_size, max_tokens, out)
+    num_seqs, num_free = cached_lens.numel(), free_blocks.numel()
+    if out is None:
+        out = paged_slots_buffers(num_seqs, max_tokens, device)
+    starts, kv_lens, slot_map, taken = out
+    int32 = torch.int32
+    _vector(cached_lens, num_seqs, device, int32, "cached_lens")
+    _vector(new_lens, num_seqs, device, int32, "new_lens")
+    _vector(free_blocks, num_free, device, int32, "free_blocks")
+    _vector(starts, num_seqs + 1, device, int32, "query_starts")
+    _vector(kv_lens, num_seqs, device, int32, "kv_lens")
+    _vector(slot_map, max_tokens, device, torch.int64, "slot_map")
+    _vector(taken, 1, device, int32, "blocks_taken")
     width, stride = _table(block_table, num_seqs, device)
-    with _on(device):
-        if out is None:
-            out = paged_slots_buffers(num_seqs, max_tokens, device)
-        _int32(out.query_starts, "query_starts", (num_seqs + 1,), device)
-        _int32(out.kv_lens, "kv_lens", (num_seqs,), device)
-        _int32(out.blocks_taken, "blocks_taken", (1,), device)
-        slots = out.slot_map
-        _need(slots.dtype == torch.int64 and slots.device == device and tuple(slots.shape) == (max_tokens,)
-              and slots.is_contiguous(), f"slot_map must be a contiguous int64 tensor [{max_tokens}] on {device}")
-        launch_paged_slots(cached_lens, new_lens, block_table, free_blocks, out.query_starts, out.kv_lens, slots,
-                           out.blocks_taken, num_seqs, width, stride, free_blocks.shape[0], block_size, max_tokens)
+    launch_paged_slots(cached_lens, new_lens, block_table, free_blocks, starts, kv_lens, slot_map, taken, num_seqs, width,
+                       stride, num_free, block_size, max_tokens)
     return out
 
 
 def paged_append(k, v, slot_map, cache: PagedCache) -> None:
     """New rows k, v [tokens, heads_kv, head_dim] into the cache's slots slot_map
     (int64 [tokens]; negative or past the cache: skipped)."""
-    import torch
-
-    shape = (slot_map.shape[0], cache.heads_kv, cache.head_dim)
-    for x, name in ((k, "k"), (v, "v")):
-        _need(tuple(x.shape) == shape and x.dtype == cache.dtype and x.device == cache.device,
-              f"{name} must be a {cache.dtype} tensor {list(shape)} on {cache.device}")
-    _need(slot_map.dtype == torch.int64 and slot_map.device == cache.device and slot_map.dim() == 1
-          and slot_map.is_contiguous(), f"slot_map must be a contiguous int64 vector on {cache.device}")
-    with _on(cache.device):
-        launch_paged_append(k, v, slot_map, cache, shape[0], _row_strides(k, "k"), _row_strides(v, "v"))
-
-
-def _workspace(workspace, nbytes: int, device):
-    """(workspace, its bytes): the caller's, or a new one."""
-    import torch
-
-    if workspace is None:
-        if nbytes == 0:
-            return None, 0
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _need(workspace.device == device and workspace.is_contiguous(), f"workspace must be a contiguous tensor on {device}")
-    have = workspace.numel() * workspace.element_size()
-    _need(have >= nbytes, f"workspace holds {have} bytes, {nbytes} are needed")
-    return workspace, have
+    device = cache.device
+    if _elsewhere(device):
+        with _torch.cuda.device(device):
+            return paged_append(k, v, slot_map, cache)
+    tokens = slot_map.numel()
+    _vector(slot_map, tokens, device, _torch.int64, "slot_map")
+    shape = (tokens, cache.heads_kv, cache.head_dim)
+    for x in (k, v):
+        if tuple(x.shape) != shape or x.dtype != cache.dtype or x.device != device:
+            raise ValueError(f"k and v must be {cache.dtype} tensors {list(shape)} on {device}")
+    launch_paged_append(k, v, slot_map, cache, tokens, _strides_of(k, "k"), _strides_of(v, "v"))
 
 
 def attention_paged_workspace(q, cache: PagedCache, num_seqs: int, max_query_len: int, max_kv_len: int):
     """A workspace for attention_paged calls of these sizes (None: they need none)."""
-    import torch
-
-    with _on(q.device):
+    with _torch.cuda.device(q.device):
         n = attention_paged_workspace_bytes(q.shape[0], num_seqs, q.shape[1], cache.heads_kv, cache.head_dim, max_query_len,
                                             max_kv_len)
-        return torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        return _torch.empty(n, dtype=_torch.uint8, device=q.device) if n else None
 
 
 def attention_paged(q, cache: PagedCache, block_table, query_starts, kv_lens, max_query_len: int,
@@ -292,37 +298,51 @@ def attention_paged(q, cache: PagedCache, block_table, query_starts, kv_lens, ma
     table's width) only decides how the work is split. `workspace`: from
     attention_paged_workspace, one per call that may run at the same time; a new one
     if not given. Returns O, like q."""
-    import torch
-
     device = cache.device
-    _need(q.dim() == 3 and q.shape[2] == cache.head_dim and q.dtype == cache.dtype and q.device == device,
-          f"q must be a {cache.dtype} tensor [tokens, heads, {cache.head_dim}] on {device}")
+    if _elsewhere(device):
+        with _torch.cuda.device(device):
+            return attention_paged(q, cache, block_table, query_starts, kv_lens, max_query_len, max_kv_len, causal, out,
+                                   workspace)
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.dtype != cache.dtype or q.device != device:
+        raise ValueError(f"q must be a {cache.dtype} tensor [tokens, heads, {cache.head_dim}] on {device}")
     tokens, heads, head_dim = q.shape
-    _need(kv_lens.dim() == 1, "kv_lens must be a vector")
-    num_seqs = kv_lens.shape[0]
-    _int32(kv_lens, "kv_lens", (num_seqs,), device)
-    _int32(query_starts, "query_starts", (num_seqs + 1,), device)
+    num_seqs = kv_lens.numel()
+    _vector(kv_lens, num_seqs, device, _torch.int32, "kv_lens")
+    _vector(query_starts, num_seqs + 1, device, _torch.int32, "query_starts")
     width, stride = _table(block_table, num_seqs, device)
     if max_kv_len is None:
         max_kv_len = width * cache.block_size
-    with _on(device):
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device, "out must be like q")
-        nbytes = attention_paged_workspace_bytes(tokens, num_seqs, heads, cache.heads_kv, head_dim, max_query_len, max_kv_len)
-        workspace, have = _workspace(workspace, nbytes, device)
-        if not launch_attention_paged(q, cache, out, workspace, have, block_table, query_starts, kv_lens, num_seqs, tokens,
-                                      heads, width, stride, max_query_len, max_kv_len, causal, _row_strides(q, "q"),
-                                      _row_strides(out, "out")):
-            raise ValueError(f"head_dim {head_dim} is not supported")
+    if out is None:
+        out = _torch.empty_like(q, memory_format=_torch.contiguous_format)
+    else:
+        _like_q(out, q)
+
+    def need():
+        return attention_paged_workspace_bytes(tokens, num_seqs, heads, cache.heads_kv, head_dim, max_query_len, max_kv_len)
+
+    given = workspace
+    if workspace is None:
+        have = need()
+        if have:
+            workspace = _torch.empty(have, dtype=_torch.uint8, device=device)
+    else:
+        have = _workspace_room(workspace, device)
+    try:
+        ok = launch_attention_paged(q, cache, out, workspace, have, block_table, query_starts, kv_lens, num_seqs, tokens,
+                                    heads, width, stride, max_query_len, max_kv_len, causal, _strides_of(q, "q"),
+                                    _strides_of(out, "out"))
+    except _fa.FaError:
+        _too_small(given, have, need())
+        raise
+    if not ok:
+        raise ValueError(f"head_dim {head_dim} is not supported")
     return out
 
 
 def attention_cross_workspace(q, k):
     """A workspace for attention_cross calls of these shapes (None: they need none)."""
-    import torch
-
-    with _on(q.device):
+    torch = _torch or _bind()
+    with torch.cuda.device(q.device):
         n = attention_cross_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
         return torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
 
@@ -334,26 +354,44 @@ def attention_cross(q, k, v, kv_lens=None, out=None, workspace=None):
     entry; what lies behind them is padding. A row without states is 0. `workspace`:
     from attention_cross_workspace, one per call that may run at the same time; a new
     one if not given. Returns O, like q."""
-    import torch
-
+    torch = _torch or _bind()
     device = q.device
-    dtype = _dtype_id(q.dtype)
-    _need(q.dim() == 4 and k.dim() == 4 and k.shape == v.shape, "q, k, v: [batch, heads, length, head_dim]")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return attention_cross(q, k, v, kv_lens, out, workspace)
+    dtype = q.dtype
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("q, k, v: [batch, heads, length, head_dim], k and v alike")
     batch, heads, q_len, head_dim = q.shape
-    heads_kv, kv_len = k.shape[1], k.shape[2]
-    _need(k.shape[0] == batch and k.shape[3] == head_dim, "q, k and v differ in batch or head_dim")
-    for x, name in ((k, "k"), (v, "v")):
-        _need(x.dtype == q.dtype and x.device == device, f"{name} must be a {q.dtype} tensor on {device}")
+    k_batch, heads_kv, kv_len, k_dim = k.shape
+    if k_batch != batch or k_dim != head_dim:
+        raise ValueError("q, k and v differ in batch or head_dim")
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
+        raise ValueError("q, k and v differ in type or device")
     if kv_lens is not None:
-        _int32(kv_lens, "kv_lens", (batch,), device)
-    with _on(device):
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == device, "out must be like q")
-        nbytes = attention_cross_workspace_bytes(batch, heads, heads_kv, q_len, kv_len, head_dim)
-        workspace, have = _workspace(workspace, nbytes, device)
-        if not launch_attention_cross(q, k, v, out, workspace, have, kv_lens, batch, heads, heads_kv, q_len, kv_len, head_dim,
-                                      dtype, _head_strides(q, "q"), _head_strides(k, "k"), _head_strides(v, "v"),
-                                      _head_strides(out, "out")):
-            raise ValueError(f"head_dim {head_dim} is not supported")
+        _vector(kv_lens, batch, device, torch.int32, "kv_lens")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        _like_q(out, q)
+
+    def need():
+        return attention_cross_workspace_bytes(batch, heads, heads_kv, q_len, kv_len, head_dim)
+
+    given = workspace
+    if workspace is None:
+        have = need()
+        if have:
+            workspace = torch.empty(have, dtype=torch.uint8, device=device)
+    else:
+        have = _workspace_room(workspace, device)
+    try:
+        ok = launch_attention_cross(q, k, v, out, workspace, have, kv_lens, batch, heads, heads_kv, q_len, kv_len, head_dim,
+                                    _dtype_id(dtype), _strides_of(q, "q"), _strides_of(k, "k"), _strides_of(v, "v"),
+                                    _strides_of(out, "out"))
+    except _fa.FaError:
+        _too_small(given, have, need())
+        raise
+    if not ok:
+        raise ValueError(f"head_dim {head_dim} is not supported")
     return out
