@@ -20,6 +20,7 @@
 #include <cmath>
 #include <cstdint>
 
+#include "fa_fused_schedule.hpp"
 #include "fa_paged.hpp"
 #include "fa_serving_core.hpp"
 
@@ -145,219 +146,183 @@ __device__ __forceinline__ long long part_row(const Args& a, const Block& b, int
     return t * (static_cast<long long>(a.heads_kv) * a.group) + b.head * a.group + h;
 }
 
-template <typename T, int D, int kWaves, bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) void serving_attention_kernel(const Args a)
+// Where a block's keys lie. Sixteen keys from a multiple of 16 on lie in one
+// page, so a copy's descriptor is scalar: the page's number comes through the
+// scalar cache (the table is constant during a launch), a step before it is used.
+template <int D, bool kPaged>
+struct Keys
 {
-    using E = Elem<T>;
-    using x8 = typename E::x8;
-    using C = TileCopy<D, kWaves>;
-    constexpr int R = 32 * kWaves;
-    constexpr int kStages = 3;
-    constexpr int kTile = kTileKeys * D;  // elements
-    __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStages * kTile];
+    typedef const __attribute__((address_space(4))) int ConstInt;
 
-    const int lane = threadIdx.x & 63;
-    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-    const int i = lane & 31;
-    const int h = lane >> 5;
-
-    const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.heads_kv));
-    const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.heads_kv));
-    const int split = rest % a.splits;
-    // Late rows see the most keys: they start first.
-    const int slot = a.slots - 1 - rest / a.splits;
-    Block b;
-    if (!find_block<R, kPaged>(a, slot, head, b)) return;
-    if (split >= b.splits) return;
-
-    // The lane's row; lanes past the last row repeat it and store nothing.
-    const int row = b.row0 + 32 * wave + i;
-    const int row_in = min(row, b.rows - 1);
-    const int token = row_in / a.group;
-    const int qh = row_in % a.group;
-    const int limit = limit_of(a, b, token);
-
-    const int k_begin = split * a.chunk;
-    const int k_end = split == b.splits - 1 ? b.end : k_begin + a.chunk;
-    const int t_begin = k_begin / kTileKeys;
-    const int t_end = (k_end + kTileKeys - 1) / kTileKeys;  // == t_begin where nothing is seen
-    // Tiles of this wave: up to its last row's limit, masked from its first row's on.
-    const int row_last = min(b.row0 + 32 * wave + 31, b.rows - 1);
-    const int wave_end = b.row0 + 32 * wave < b.rows ? limit_of(a, b, row_last / a.group) : 0;
-    const int t_last = min(t_end, (wave_end + kTileKeys - 1) / kTileKeys);
-    const int t_mask = limit_of(a, b, min(b.row0 + 32 * wave, b.rows - 1) / a.group) / kTileKeys;
-
-    // Byte offset of 16 keys from `key` on, and the bytes of them that exist: a
-    // copy's rows past those read as zero, and so does a page that the cache
-    // does not have.
-    const uint32_t k_row_bytes = static_cast<uint32_t>(a.k_row * 2);
-    const uint32_t v_row_bytes = static_cast<uint32_t>(a.v_row * 2);
-    int pages = 0, pages_base = -1;  // lane l: entry pages_base + l of the block table
-    const uint64_t k_bytes = uniform(reinterpret_cast<uint64_t>(a.k) + static_cast<uint64_t>(b.head * a.k_head * 2) +
-                                     (kPaged ? 0 : static_cast<uint64_t>(b.seq * a.k_seq * 2)));
-    const uint64_t v_bytes = uniform(reinterpret_cast<uint64_t>(a.v) + static_cast<uint64_t>(b.head * a.v_head * 2) +
-                                     (kPaged ? 0 : static_cast<uint64_t>(b.seq * a.v_seq * 2)));
+    // Sixteen keys: byte addresses of the first and the rows of them that exist;
+    // the others of a copy read as zero, and so does a page outside the cache.
     struct Half
     {
         uint64_t k, v;
         int rows;
     };
-    auto half_at = [&](int key) {
+
+    const Args& a;
+    uint64_t k_base, v_base;
+    uint64_t table;
+    int end;
+
+    __device__ __forceinline__ Keys(const Args& args, const Block& b) : a(args), end(b.end)
+    {
+        k_base = reinterpret_cast<uint64_t>(a.k) + static_cast<uint64_t>(b.head * a.k_head * 2);
+        v_base = reinterpret_cast<uint64_t>(a.v) + static_cast<uint64_t>(b.head * a.v_head * 2);
+        if constexpr (!kPaged)
+        {
+            k_base += static_cast<uint64_t>(b.seq * a.k_seq * 2);
+            v_base += static_cast<uint64_t>(b.seq * a.v_seq * 2);
+        }
+        k_base = uniform(k_base);
+        v_base = uniform(v_base);
+        table = uniform(reinterpret_cast<uint64_t>(a.table) + static_cast<uint64_t>(b.seq * a.table_stride * 4));
+    }
+
+    // The page that holds `key` (the last one of the row for a key past it).
+    // Only where the block sees a key, so the row has an entry.
+    __device__ __forceinline__ int page_of(int key) const
+    {
+        if constexpr (!kPaged) return 0;
+        const unsigned entry = static_cast<unsigned>(min(key >> a.block_shift, a.table_width - 1));
+        return *reinterpret_cast<ConstInt*>(table + static_cast<uint64_t>(entry) * 4);
+    }
+
+    __device__ __forceinline__ Half half_at(int key, int page) const
+    {
         Half r;
-        r.rows = max(0, min(16, b.end - key));
+        r.rows = max(0, min(16, end - key));
         if constexpr (kPaged)
         {
-            const int entry = key >> a.block_shift;
-            if ((entry & ~63) != pages_base)
-            {
-                pages_base = entry & ~63;
-                const int e = pages_base + lane;
-                pages = e < a.table_width ? a.table[b.seq * a.table_stride + e] : -1;
-            }
-            const int page = __builtin_amdgcn_readlane(pages, entry & 63);
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_blocks)) r.rows = 0;
-            const long long in_page = key & ((1 << a.block_shift) - 1);
-            const long long p = r.rows ? page : 0;
-            r.k = k_bytes + static_cast<uint64_t>((p * a.k_seq + in_page * a.k_row) * 2);
-            r.v = v_bytes + static_cast<uint64_t>((p * a.v_seq + in_page * a.v_row) * 2);
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_blocks)) r.rows = page = 0;
+            const int in_page = key & ((1 << a.block_shift) - 1);
+            const uint64_t off = (static_cast<uint64_t>(page) * static_cast<uint64_t>(a.k_seq) +
+                                  static_cast<uint64_t>(in_page) * static_cast<uint64_t>(a.k_row)) * 2;
+            r.k = k_base + off;
+            r.v = v_base + off;
         }
         else
         {
-            r.k = k_bytes + static_cast<uint64_t>(key * a.k_row * 2);
-            r.v = v_bytes + static_cast<uint64_t>(key * a.v_row * 2);
+            r.k = k_base + static_cast<uint64_t>(key) * static_cast<uint64_t>(a.k_row * 2);
+            r.v = v_base + static_cast<uint64_t>(key) * static_cast<uint64_t>(a.v_row * 2);
         }
         return r;
-    };
-    auto descriptor = [&](uint64_t base, int rows, uint32_t row_bytes) {
+    }
+
+    static __device__ __forceinline__ i32x4 descriptor(uint64_t base, int rows, uint32_t row_bytes)
+    {
         i32x4 r;
         r[0] = uniform(static_cast<int>(static_cast<uint32_t>(base)));
         r[1] = uniform(static_cast<int>(static_cast<uint32_t>(base >> 32) & 0xffffu));
         r[2] = uniform(rows > 0 ? static_cast<int>((rows - 1) * row_bytes + D * 2) : 0);
         r[3] = static_cast<int>(fa::kRawBufferConfig);
         return r;
-    };
-    // A copy's lanes: row and chunk of each lane's 16 bytes, from the half's first row.
-    uint32_t koff[C::kIssues], voff[C::kIssues];
-    {
-        const int sub = (lane % C::kLanes) / C::kChunks;
-        const int pchunk = lane % C::kChunks;
-#pragma unroll
-        for (int u = 0; u < C::kIssues; ++u)
-        {
-            const int r = (u * kWaves + wave) * C::kRows + sub;
-            koff[u] = static_cast<uint32_t>(r & 15) * k_row_bytes + ((pchunk ^ swz_k<D>(r)) * 16);
-            voff[u] = static_cast<uint32_t>(r & 15) * v_row_bytes + ((pchunk ^ swz_v<D>(r)) * 16);
-        }
-    }
-    const uint32_t lds_base = fa::lds_addr(lds);
-    auto copy_tile = [&](int t) {
-        const int stage = t % kStages;
-        const Half lo = half_at(t * kTileKeys), hi = half_at(t * kTileKeys + 16);
-#pragma unroll
-        for (int u = 0; u < C::kIssues; ++u)
-        {
-            const int r0 = (u * kWaves + wave) * C::kRows;
-            const uint64_t kb = r0 < 16 ? lo.k : hi.k, vb = r0 < 16 ? lo.v : hi.v;
-            const int rows = r0 < 16 ? lo.rows : hi.rows;
-            const uint32_t at = lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes;
-            const i32x4 kd = descriptor(kb, rows, k_row_bytes);
-            const i32x4 vd = descriptor(vb, rows, v_row_bytes);
-            if (C::kLanes == 64 || lane < C::kLanes)
-            {
-                fa::dma16(kd, koff[u], at);
-                fa::dma16(vd, voff[u], at + kStages * kTile * 2);
-            }
-        }
-    };
-
-    copy_tile(t_begin);
-    copy_tile(t_begin + 1);
-
-    x8 qr[D / 16];
-    {
-        const uint16_t* qp = a.q + (kPaged ? (b.first_token + static_cast<long long>(token)) * a.q_row
-                                           : b.seq * a.q_seq + token * a.q_row) +
-                             (b.head * a.group + qh) * a.q_head;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) qr[ks] = *reinterpret_cast<const x8*>(qp + 16 * ks + 8 * h);
-    }
-    int k_at[D / 16], v_at[D / 32];
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) k_at[ks] = i * D + (((2 * ks + h) ^ swz_k<D>(i)) << 3);
-    {
-        const int g16 = lane >> 4, s16 = lane & 15;
-        const int vr = 4 * (g16 >> 1) + (s16 >> 2);
-        const int dim = 16 * (g16 & 1) + 4 * (s16 & 3);
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db)
-        {
-            const int col = 32 * db + dim;
-            v_at[db] = kStages * kTile + vr * D + (((col >> 3) ^ swz_v<D>(vr)) << 3) + (col & 7);
-        }
     }
 
-    f32x16 o[D / 32];
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
-    float m = kEmptyBase, l = 0.0f;
-
-    for (int t = t_begin; t < t_end; ++t)
+    // Element offset of a lane's key below `end`, for the rare paths that read
+    // keys outside the pipeline; false: it holds zeros.
+    __device__ __forceinline__ bool lane_key(int key, uint64_t& k, uint64_t& v) const
     {
-        // Tile t has landed once only tile t+1's copies are in flight; past the
-        // barrier every wave has left tile t-1, whose stage takes tile t+2.
-        fa::wait_vm_lgkm0<2 * C::kIssues>();
-        barrier();
-        copy_tile(t + 2);
-        if (t >= t_last) continue;
-        const uint16_t* const stage = lds + (t % kStages) * kTile;
-        f32x16 s = {};
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) s = E::mfma(*reinterpret_cast<const x8*>(stage + k_at[ks]), qr[ks], s);
-        if (t >= t_mask) mask_tile(s, limit - t * kTileKeys - 4 * h);
-        const float m_new = __builtin_elementwise_maximum(m, row_max_raw(s) * a.c_log2 - E::kBias);
-        if (__any(m_new != m))
+        bool there = key < end;
+        int page = 0;
+        if constexpr (kPaged)
         {
-            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-            l *= alpha;
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-            m = m_new;
+            if (there) page = *reinterpret_cast<const int*>(table + static_cast<uint64_t>(key >> a.block_shift) * 4);
+            there = there && static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
         }
-        x8 p[2];
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-        {
-#pragma clang fp contract(off)
-            // The product is rounded as the base was: the largest score's weight
-            // is exactly 2^kBias however large the score.
-            const float x = s[r] * a.c_log2 - m;
-            p[r >> 3][r & 7] = static_cast<T>(__builtin_amdgcn_exp2f(x));
-        }
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) l = E::add_pair(p[r >> 3][r & 7], p[r >> 3][(r & 7) + 1], l);
-#pragma unroll
-        for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db)
-            {
-                const uint16_t* base = stage + v_at[db] + mm * 16 * D;
-                const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base));
-                const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(base + 8 * D));
-                o[db] = E::mfma(__builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), p[mm],
-                                o[db]);
-            }
+        const Half r = half_at(key, there ? page : 0);
+        k = r.k;
+        v = r.v;
+        return there;
     }
-    fa::wait_vm_lgkm0<0>();  // the last copies have landed before the workgroup's LDS goes
+};
 
+// The rows of a wave and what its lanes see of the keys.
+struct Rows
+{
+    int row;      // the lane's row (at or past Block::rows: none)
+    int token, qh;
+    int limit;    // keys the lane's row sees; lanes past the last row repeat it
+    int t_begin, t_end;  // the workgroup's tiles (equal where nothing is seen)
+    int t_last;   // the wave's tiles end here
+    int t_mask;   // first tile that some lane does not see whole
+};
+
+template <int R>
+__device__ __forceinline__ Rows wave_rows(const Args& a, const Block& b, int split, int wave, int i)
+{
+    Rows r;
+    r.row = b.row0 + 32 * wave + i;
+    const int row_in = min(r.row, b.rows - 1);
+    r.token = row_in / a.group;
+    r.qh = row_in - r.token * a.group;
+    r.limit = limit_of(a, b, r.token);
+    const int k_begin = split * a.chunk;
+    const int k_end = split == b.splits - 1 ? b.end : k_begin + a.chunk;
+    r.t_begin = k_begin / kTileKeys;
+    r.t_end = (k_end + kTileKeys - 1) / kTileKeys;
+    const int first = b.row0 + 32 * wave;
+    const int wave_end = first < b.rows ? limit_of(a, b, min(first + 31, b.rows - 1) / a.group) : 0;
+    r.t_last = min(r.t_end, (wave_end + kTileKeys - 1) / kTileKeys);
+    r.t_mask = limit_of(a, b, min(first, b.rows - 1) / a.group) / kTileKeys;
+    return r;
+}
+
+template <bool kPaged>
+__device__ __forceinline__ long long q_offset(const Args& a, const Block& b, const Rows& r)
+{
+    return (kPaged ? (b.first_token + static_cast<long long>(r.token)) * a.q_row : b.seq * a.q_seq + r.token * a.q_row) +
+           (b.head * a.group + r.qh) * a.q_head;
+}
+
+template <bool kPaged>
+__device__ __forceinline__ long long o_offset(const Args& a, const Block& b, int token, int qh)
+{
+    return (kPaged ? (b.first_token + static_cast<long long>(token)) * a.o_row : b.seq * a.o_seq + token * a.o_row) +
+           (b.head * a.group + qh) * a.o_head;
+}
+
+// Per-lane LDS element offsets of a tile's operand reads.
+template <int D>
+__device__ __forceinline__ int k_read_offset(int i, int h, int ks)
+{
+    return i * D + (((2 * ks + h) ^ swz_k<D>(i)) << 3);
+}
+template <int D>
+__device__ __forceinline__ int v_read_offset(int lane, int db)
+{
+    const int g16 = lane >> 4, s16 = lane & 15;
+    const int row = 4 * (g16 >> 1) + (s16 >> 2);
+    const int col = 32 * db + 16 * (g16 & 1) + 4 * (s16 & 3);
+    return row * D + (((col >> 3) ^ swz_v<D>(row)) << 3) + (col & 7);
+}
+
+// A V operand: keys 16*half .. of head dims 32*db .. (`base`: the stage plus the
+// lane's offset for db, in elements).
+template <typename T, int D>
+__device__ __forceinline__ typename Elem<T>::x8 read_v(const uint16_t* base, int half)
+{
+    const uint16_t* at = base + half * 16 * D;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 8 * D));
+    return __builtin_bit_cast(typename Elem<T>::x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The lane's row of O: normalised to the element type, or the partial result of
+// one chunk.
+template <typename T, int D, bool kPaged>
+__device__ __forceinline__ void store_row(const Args& a, const Block& b, const Rows& r, int split, int h,
+                                          const f32x16 (&o)[D / 32], float m, float l)
+{
     float la, lb;
     row_halves(l, la, lb);
     l = la + lb;
-    if (row >= b.rows) return;
+    if (r.row >= b.rows) return;
     if (b.splits > 1)
     {
-        const long long pr = part_row<kPaged>(a, b, token, qh) * a.splits + split;
+        const long long pr = part_row<kPaged>(a, b, r.token, r.qh) * a.splits + split;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -373,9 +338,7 @@ __global__ __launch_bounds__(64 * kWaves) void serving_attention_kernel(const Ar
     }
     // A row that saw nothing has the sum 0 and gives 0; a NaN sum leaves O's NaN.
     const float inv = l > 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f;
-    uint16_t* op = a.o + (kPaged ? (b.first_token + static_cast<long long>(token)) * a.o_row
-                                 : b.seq * a.o_seq + token * a.o_row) +
-                   (b.head * a.group + qh) * a.o_head;
+    uint16_t* op = a.o + o_offset<kPaged>(a, b, r.token, r.qh);
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
@@ -386,6 +349,487 @@ __global__ __launch_bounds__(64 * kWaves) void serving_attention_kernel(const Ar
             w.y = pack_pair<T>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
             *reinterpret_cast<uint2*>(op + 32 * db + 8 * g + 4 * h) = w;
         }
+}
+
+// The block and the chunk of this workgroup; false: nothing to do.
+template <int R, bool kPaged>
+__device__ __forceinline__ bool take_block(const Args& a, Block& b, int& split)
+{
+    const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.heads_kv));
+    const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.heads_kv));
+    split = rest % a.splits;
+    // Late rows see the most keys: they start first.
+    return find_block<R, kPaged>(a, a.slots - 1 - rest / a.splits, head, b) && split < b.splits;
+}
+
+// Few rows (one or two waves of them): bound by the reads of K and V. A step takes
+// one tile, with the copies of the next two in flight.
+template <typename T, int D, int kWaves, bool kPaged>
+__global__ __launch_bounds__(64 * kWaves) void serving_few_rows_kernel(const Args a)
+{
+    using E = Elem<T>;
+    using x8 = typename E::x8;
+    using C = TileCopy<D, kWaves>;
+    constexpr int R = 32 * kWaves;
+    constexpr int kStages = 3;
+    constexpr int kTile = kTileKeys * D;  // elements
+    __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStages * kTile];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int i = lane & 31;
+    const int h = lane >> 5;
+    Block b;
+    int split;
+    if (!take_block<R, kPaged>(a, b, split)) return;
+    const Rows r = wave_rows<R>(a, b, split, wave, i);
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+    float m = kEmptyBase, l = 0.0f;
+    if (r.t_begin < r.t_end)
+    {
+        const Keys<D, kPaged> keys(a, b);
+        const uint32_t k_row_bytes = static_cast<uint32_t>(a.k_row * 2);
+        const uint32_t v_row_bytes = static_cast<uint32_t>(a.v_row * 2);
+        // A copy's lanes: row and chunk of each lane's 16 bytes, from the half's first row.
+        uint32_t koff[C::kIssues], voff[C::kIssues];
+        {
+            const int sub = (lane % C::kLanes) / C::kChunks;
+            const int pchunk = lane % C::kChunks;
+#pragma unroll
+            for (int u = 0; u < C::kIssues; ++u)
+            {
+                const int row = (u * kWaves + wave) * C::kRows + sub;
+                koff[u] = static_cast<uint32_t>(row & 15) * k_row_bytes + ((pchunk ^ swz_k<D>(row)) * 16);
+                voff[u] = static_cast<uint32_t>(row & 15) * v_row_bytes + ((pchunk ^ swz_v<D>(row)) * 16);
+            }
+        }
+        const uint32_t lds_base = fa::lds_addr(lds);
+        int page_lo = keys.page_of(r.t_begin * kTileKeys), page_hi = keys.page_of(r.t_begin * kTileKeys + 16);
+        auto copy_tile = [&](int t) {
+            const int stage = t % kStages;
+            const auto lo = keys.half_at(t * kTileKeys, page_lo), hi = keys.half_at(t * kTileKeys + 16, page_hi);
+            page_lo = keys.page_of((t + 1) * kTileKeys);
+            page_hi = keys.page_of((t + 1) * kTileKeys + 16);
+#pragma unroll
+            for (int u = 0; u < C::kIssues; ++u)
+            {
+                const bool low = (u * kWaves + wave) * C::kRows < 16;
+                const uint32_t at = lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes;
+                fa::dma16(keys.descriptor(low ? lo.k : hi.k, low ? lo.rows : hi.rows, k_row_bytes), koff[u], at);
+                fa::dma16(keys.descriptor(low ? lo.v : hi.v, low ? lo.rows : hi.rows, v_row_bytes), voff[u],
+                          at + kStages * kTile * 2);
+            }
+        };
+        static_assert(C::kLanes == 64, "whole copies");
+
+        copy_tile(r.t_begin);
+        copy_tile(r.t_begin + 1);
+
+        x8 qr[D / 16];
+        const uint16_t* qp = a.q + q_offset<kPaged>(a, b, r);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qr[ks] = *reinterpret_cast<const x8*>(qp + 16 * ks + 8 * h);
+
+        for (int t = r.t_begin; t < r.t_end; ++t)
+        {
+            // Tile t has landed once only tile t+1's copies are in flight; past the
+            // barrier every wave has left tile t-1, whose stage takes tile t+2.
+            fa::wait_vm_lgkm0<2 * C::kIssues>();
+            barrier();
+            copy_tile(t + 2);
+            if (t >= r.t_last) continue;
+            const uint16_t* const stage = lds + (t % kStages) * kTile;
+            f32x16 s = {};
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+                s = E::mfma(*reinterpret_cast<const x8*>(stage + k_read_offset<D>(i, h, ks)), qr[ks], s);
+            if (t >= r.t_mask) mask_tile(s, r.limit - t * kTileKeys - 4 * h);
+            const float m_new = __builtin_elementwise_maximum(m, row_max_raw(s) * a.c_log2 - E::kBias);
+            if (__any(m_new != m))
+            {
+                const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+                l *= alpha;
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+                m = m_new;
+            }
+            x8 p[2];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+            {
+#pragma clang fp contract(off)
+                // The product is rounded as the base was: the largest score's weight
+                // is exactly 2^kBias however large the score.
+                const float x = s[e] * a.c_log2 - m;
+                p[e >> 3][e & 7] = static_cast<T>(__builtin_amdgcn_exp2f(x));
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) l = E::add_pair(p[e >> 3][e & 7], p[e >> 3][(e & 7) + 1], l);
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db)
+                    o[db] = E::mfma(read_v<T, D>(stage + kStages * kTile + v_read_offset<D>(lane, db), half), p[half], o[db]);
+        }
+        fa::wait_vm_lgkm0<0>();  // the last copies have landed before the workgroup's LDS goes
+    }
+    store_row<T, D, kPaged>(a, b, r, split, h, o, m, l);
+}
+
+// Keeps a value's producing instructions inside the current block: the compiler
+// cannot sink them past the next branch.
+__device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void pin(int& x) { asm volatile("" : "+v"(x)); }
+template <typename x8>
+__device__ __forceinline__ void pin8(x8& x)
+{
+    i32x4 bits = __builtin_bit_cast(i32x4, x);
+    asm volatile("" : "+v"(bits));
+    x = __builtin_bit_cast(x8, bits);
+}
+
+// Weights of scores s[kFirst + e], e < 8, against base m into p[e]; their rounded
+// values are added to `sum`. kRounded: the product is rounded before the base is
+// subtracted, so the score that set the base weighs exactly 2^kBias whatever its
+// size; else one fused multiply-add.
+template <typename T, bool kRounded>
+__device__ __forceinline__ void weigh(const f32x16& s, int first, typename Elem<T>::x8& p, float m, float c_log2, float& sum)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+    {
+        float x;
+        if constexpr (kRounded)
+        {
+#pragma clang fp contract(off)
+            x = s[first + e] * c_log2 - m;
+        }
+        else x = fmaf(s[first + e], c_log2, -m);
+        p[e] = static_cast<T>(__builtin_amdgcn_exp2f(x));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) sum = Elem<T>::add_pair(p[e], p[e + 1], sum);
+}
+
+// Many rows (128 or 256 of a key head): bound by the matrix cores, beside which
+// the exponentials have to hide. The step of the fused self-attention kernel: in
+// block A the matrix cores compute tile j+1's scores while the vector unit ends
+// tile j's exponentials; past the step's one barrier, in block B, they add tile j's
+// P V while the vector unit starts tile j+1's. K is copied three tiles ahead, V two.
+// The base is not followed tile by tile: it is set by the first tile and moved only
+// when a tile's row sum passes kSumLimit, which bounds every weight (2^48 in bf16;
+// 2^15 in fp16, whose largest value is near 2^16). The move is rare; it recomputes
+// the tile's scores from memory.
+template <typename T>
+constexpr float kSumLimit = 281474976710656.0f;  // 2^48
+template <>
+constexpr float kSumLimit<_Float16> = 32768.0f;
+// From here on the fused product's rounding against the base is no longer small
+// (fp32's spacing at 2^28 is 32): every tile takes the exact path.
+constexpr float kCoarseBase = 268435456.0f;
+
+template <typename T, int D, int kWaves, bool kPaged>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 8))) void serving_many_rows_kernel(
+    const Args a)
+{
+    using E = Elem<T>;
+    using x8 = typename E::x8;
+    using C = TileCopy<D, kWaves>;
+    constexpr int R = 32 * kWaves;
+    constexpr int kStages = fa::kFusedStages;
+    static_assert(kStages == 3, "the step's copies run three K and two V tiles ahead");
+    constexpr int kTile = kTileKeys * D;  // elements
+    constexpr int kI = C::kIssues;
+    // A wave's copies of a tile lie in one half of it, or in both.
+    constexpr int kHalves = kI > 1 ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStages * kTile];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int i = lane & 31;
+    const int h = lane >> 5;
+    Block b;
+    int split;
+    if (!take_block<R, kPaged>(a, b, split)) return;
+    const Rows r = wave_rows<R>(a, b, split, wave, i);
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+    float m = kEmptyBase, l = 0.0f;
+    if (r.t_begin < r.t_end)
+    {
+        const Keys<D, kPaged> keys(a, b);
+        const float c_log2 = a.c_log2;
+        const uint32_t k_row_bytes = static_cast<uint32_t>(a.k_row * 2);
+        const uint32_t v_row_bytes = static_cast<uint32_t>(a.v_row * 2);
+        uint32_t koff[kI], voff[kI];
+        {
+            const int sub = (lane % C::kLanes) / C::kChunks;
+            const int pchunk = lane % C::kChunks;
+#pragma unroll
+            for (int u = 0; u < kI; ++u)
+            {
+                const int row = (u * kWaves + wave) * C::kRows + sub;
+                koff[u] = static_cast<uint32_t>(row & 15) * k_row_bytes + ((pchunk ^ swz_k<D>(row)) * 16);
+                voff[u] = static_cast<uint32_t>(row & 15) * v_row_bytes + ((pchunk ^ swz_v<D>(row)) * 16);
+            }
+        }
+        const uint32_t lds_base = fa::lds_addr(lds);
+        const int half0 = kHalves == 1 ? (wave * C::kRows) & 16 : 0;  // first key of the wave's (first) half
+        struct Place
+        {
+            typename Keys<D, kPaged>::Half half[kHalves];
+        };
+        int pages[kHalves];  // of the tile whose place is computed next
+        auto fetch_pages = [&](int t) {
+#pragma unroll
+            for (int x = 0; x < kHalves; ++x) pages[x] = keys.page_of(t * kTileKeys + half0 + 16 * x);
+        };
+        auto place_of = [&](int t) {
+            Place p;
+#pragma unroll
+            for (int x = 0; x < kHalves; ++x) p.half[x] = keys.half_at(t * kTileKeys + half0 + 16 * x, pages[x]);
+            return p;
+        };
+        auto copy = [&](uint64_t base, int rows, uint32_t row_bytes, uint32_t off, uint32_t at) {
+            const i32x4 d = keys.descriptor(base, rows, row_bytes);
+            if constexpr (C::kLanes == 64) fa::dma16(d, off, at);
+            else if (lane < C::kLanes) fa::dma16(d, off, at);
+        };
+        auto copy_k = [&](const Place& p, int stage, int u) {
+            const auto& half = p.half[kHalves == 1 ? 0 : (u * kWaves * C::kRows) >> 4];
+            copy(half.k, half.rows, k_row_bytes, koff[u], lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
+        };
+        auto copy_v = [&](const Place& p, int stage, int u) {
+            const auto& half = p.half[kHalves == 1 ? 0 : (u * kWaves * C::kRows) >> 4];
+            copy(half.v, half.rows, v_row_bytes, voff[u],
+                 lds_base + (kStages + stage) * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
+        };
+        static_assert(kHalves == 1 || (kWaves * C::kRows) % 16 == 0, "every wave's copy u lies in the same half");
+
+        const int t0 = r.t_begin;
+        const int cnt = r.t_end - t0;
+        const int lw = r.t_last - t0 - 1;             // last step this wave computes
+        const int j_mask = min(lw, r.t_mask - t0 - 1);  // first step whose next tile is masked
+
+        // Prologue: K 0..2 and V 0..1; `ahead` is the place of tile 3 (K next, V a step
+        // later), `behind` that of tile 2 (V next).
+        Place ahead, behind;
+        fetch_pages(t0);
+#pragma unroll
+        for (int x = 0; x < kStages; ++x)
+        {
+            const Place p = place_of(t0 + x);
+            fetch_pages(t0 + x + 1);
+#pragma unroll
+            for (int u = 0; u < kI; ++u) copy_k(p, x, u);
+            if (x < 2)
+#pragma unroll
+                for (int u = 0; u < kI; ++u) copy_v(p, x, u);
+            else behind = p;
+        }
+        ahead = place_of(t0 + 3);
+        fetch_pages(t0 + 4);
+
+        x8 qr[D / 16];
+        const uint16_t* qp = a.q + q_offset<kPaged>(a, b, r);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) qr[ks] = *reinterpret_cast<const x8*>(qp + 16 * ks + 8 * h);
+
+        int k_at[D / 16], v_at[D / 32];  // byte offsets, pinned at each use: the stage then folds into the read
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) k_at[ks] = 2 * k_read_offset<D>(i, h, ks);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) v_at[db] = 2 * (kStages * kTile + v_read_offset<D>(lane, db));
+        x8 ka[D / 16], va[D / 32][2];
+        auto load_k = [&](int stage, int first, int count) {
+#pragma unroll
+            for (int ks = first; ks < first + count; ++ks)
+            {
+                pin(k_at[ks]);
+                ka[ks] = *reinterpret_cast<const x8*>(reinterpret_cast<const char*>(lds + stage * kTile) + k_at[ks]);
+            }
+        };
+        auto load_v = [&](int stage, int first, int count) {
+#pragma unroll
+            for (int db = first; db < first + count; ++db)
+            {
+                pin(v_at[db]);
+                const uint16_t* base = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(lds + stage * kTile) + v_at[db]);
+                va[db][0] = read_v<T, D>(base, 0);
+                va[db][1] = read_v<T, D>(base, 1);
+            }
+        };
+
+        f32x16 sbuf[2];
+        x8 p_lo[2], p_hi;
+        float tsum = 0.0f;
+        int limit_bits = __builtin_bit_cast(int, kSumLimit<T>);
+        auto note_base = [&](float base) {
+            if (__any(base != kEmptyBase && __builtin_fabsf(base) >= kCoarseBase)) limit_bits = __builtin_bit_cast(int, -1.0f);
+            limit_bits = uniform(limit_bits);
+        };
+        // The first K tile: everything but K 1, K 2 and V 0, V 1 has landed.
+        fa::wait_vm_lgkm0<4 * kI>();
+        barrier();
+        if (lw >= 0)
+        {
+            load_k(0, 0, D / 16);
+            sbuf[0] = f32x16{};
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) sbuf[0] = E::mfma(ka[ks], qr[ks], sbuf[0]);
+            if (t0 >= r.t_mask) mask_tile(sbuf[0], r.limit - t0 * kTileKeys - 4 * h);
+            m = __builtin_elementwise_maximum(m, row_max_raw(sbuf[0]) * c_log2 - E::kBias);
+            weigh<T, false>(sbuf[0], 0, p_lo[0], m, c_log2, tsum);
+            note_base(m);
+        }
+        fa::wait_vm_lgkm0<0>();
+        barrier();  // every prologue tile has landed; K 0's stage is free
+        load_k(1, 0, D / 16);
+
+        // The base lags (see above): tile jj's P was zeroed; its scores again, the base
+        // at the row maximum, O and l rescaled, its P V from V's stage (intact until the
+        // next step's copies), and the first half of the next tile's exponentials again.
+        auto rebase = [&](auto par_tag, int jj) {
+            constexpr int P = decltype(par_tag)::value;
+            constexpr int B = P & 1;
+            const int t = t0 + jj;
+            uint64_t kp, vp;
+            const bool there = keys.lane_key(t * kTileKeys + i, kp, vp);
+            f32x16 st = {};
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+            {
+                const x8 kr = there ? *reinterpret_cast<const x8*>(kp + (16 * ks + 8 * h) * 2) : x8{};
+                st = E::mfma(kr, qr[ks], st);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (t >= r.t_mask) mask_tile(st, r.limit - t * kTileKeys - 4 * h);
+            const float m_new = __builtin_elementwise_maximum(m, row_max_raw(st) * c_log2 - E::kBias);
+            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            note_base(m_new);
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+            float sum = 0.0f;
+            x8 pr[2];
+            weigh<T, true>(st, 0, pr[0], m, c_log2, sum);
+            weigh<T, true>(st, 8, pr[1], m, c_log2, sum);
+            l = l * alpha + sum;
+            load_v(P % kStages, 0, D / 32);
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) o[x % (D / 32)] = E::mfma(va[x % (D / 32)][x / (D / 32)], pr[x / (D / 32)], o[x % (D / 32)]);
+            tsum = 0.0f;
+            weigh<T, false>(sbuf[B ^ 1], 0, p_lo[B ^ 1], m, c_log2, tsum);
+        };
+
+        constexpr int kChunk = kI;                  // chunks per block, one copy each
+        constexpr int kMfmaPer = (D / 16) / kChunk;  // products per chunk
+        constexpr int kVPer = (D / 32) / kChunk;
+        constexpr int kKPer = (D / 16) / kChunk;
+        static_assert(kMfmaPer * kChunk == D / 16 && kVPer * kChunk == D / 32 && 8 % kChunk == 0, "chunks");
+        constexpr int kExpPer = 8 / kChunk;
+        // kExpPer weights of a half tile of scores, as weigh.
+        auto weigh_part = [&](const f32x16& s, int first, x8& p, int at) {
+#pragma unroll
+            for (int e = at; e < at + kExpPer; ++e)
+                p[e] = static_cast<T>(__builtin_amdgcn_exp2f(fmaf(s[first + e], c_log2, -m)));
+#pragma unroll
+            for (int e = at; e < at + kExpPer; e += 2) tsum = E::add_pair(p[e], p[e + 1], tsum);
+        };
+        auto pv_part = [&](const x8 (&p)[2], int first, int count) {
+#pragma unroll
+            for (int x = first; x < first + count; ++x)
+                o[x % (D / 32)] = E::mfma(va[x % (D / 32)][x / (D / 32)], p[x / (D / 32)], o[x % (D / 32)]);
+        };
+        auto qk_part = [&](f32x16& s, int first, int count) {
+#pragma unroll
+            for (int ks = first; ks < first + count; ++ks) s = E::mfma(ka[ks], qr[ks], s);
+        };
+        auto step = [&](auto par_tag, int jj) {
+            constexpr int P = decltype(par_tag)::value;
+            constexpr int B = P & 1;
+            // Block A
+            sbuf[B ^ 1] = f32x16{};
+#pragma unroll
+            for (int c = 0; c < kChunk; ++c)
+            {
+                qk_part(sbuf[B ^ 1], c * kMfmaPer, 1);
+                __builtin_amdgcn_sched_barrier(0);
+                copy_k(ahead, P % kStages, c);
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(P % kStages, c * kVPer, kVPer);
+                qk_part(sbuf[B ^ 1], c * kMfmaPer + 1, kMfmaPer - 1);
+                weigh_part(sbuf[B], 8, p_hi, c * kExpPer);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            pin8(p_hi);
+            pin(tsum);
+            // K jj+2 and V jj+1 have landed (K jj+3 may fly), every LDS read is done.
+            fa::wait_vm_lgkm0<kI>();
+            barrier();
+            // Block B
+            const bool rare = __any(tsum > __builtin_bit_cast(float, limit_bits));
+            if (rare)
+            {
+                asm volatile("");  // a branch, not selects on the common path
+                p_lo[B] = x8{};
+                p_hi = x8{};
+                tsum = 0.0f;
+            }
+            l += tsum;
+            // Past the wave's last tile the next scores are of a stage that nobody needs.
+            if (jj >= j_mask) mask_tile(sbuf[B ^ 1], jj == lw ? -kTileKeys : r.limit - (t0 + jj + 1) * kTileKeys - 4 * h);
+            __builtin_amdgcn_sched_barrier(0);
+            const x8 p_cur[2] = {p_lo[B], p_hi};
+            tsum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kChunk; ++c)
+            {
+                pv_part(p_cur, c * kMfmaPer, 1);
+                __builtin_amdgcn_sched_barrier(0);
+                copy_v(behind, (P + 2) % kStages, c);
+                __builtin_amdgcn_sched_barrier(0);
+                load_k((P + 2) % kStages, c * kKPer, kKPer);
+                pv_part(p_cur, c * kMfmaPer + 1, kMfmaPer - 1);
+                weigh_part(sbuf[B ^ 1], 0, p_lo[B ^ 1], c * kExpPer);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            behind = ahead;
+            ahead = place_of(t0 + jj + 4);
+            fetch_pages(t0 + jj + 5);
+            pin8(p_lo[B ^ 1]);
+            pin(tsum);
+            if (rare) rebase(par_tag, jj);
+            pin(l);
+        };
+        const int active = max(0, min(cnt, lw + 1));
+        fa::fused_group_walk(active, step);
+        // The steps past this wave's last tile: its share of the copies and the barriers.
+        for (int jj = active; jj < cnt; ++jj)
+        {
+            const int stage = jj % kStages;
+#pragma unroll
+            for (int u = 0; u < kI; ++u) copy_k(ahead, stage, u);
+            fa::wait_vm_lgkm0<kI>();
+            barrier();
+#pragma unroll
+            for (int u = 0; u < kI; ++u) copy_v(behind, (stage + 2) % kStages, u);
+            behind = ahead;
+            ahead = place_of(t0 + jj + 4);
+            fetch_pages(t0 + jj + 5);
+        }
+        fa::wait_vm_lgkm0<0>();  // the last copies have landed before the workgroup's LDS goes
+    }
+    store_row<T, D, kPaged>(a, b, r, split, h, o, m, l);
 }
 
 // Joins the chunks of one row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c
@@ -447,9 +891,7 @@ __global__ __launch_bounds__(256) void serving_join_kernel(const Args a, int blo
 #pragma unroll
     for (int x = 1; x < kAtOnce; ++x) acc += sums[x * kLanes + tid];
     const float inv = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
-    uint16_t* op = a.o + (kPaged ? (b.first_token + static_cast<long long>(token)) * a.o_row
-                                 : b.seq * a.o_seq + token * a.o_row) +
-                   (b.head * a.group + qh) * a.o_head;
+    uint16_t* op = a.o + o_offset<kPaged>(a, b, token, qh);
     uint2 w;
     w.x = pack_pair<T>(acc[0] * inv, acc[1] * inv);
     w.y = pack_pair<T>(acc[2] * inv, acc[3] * inv);
@@ -508,8 +950,10 @@ int launch_typed(const Args& a, const Plan& p, int head_rows, hipStream_t stream
     const int block_rows = std::min(32 * kWaves, head_rows);
     const long long join_blocks = p.slots * a.heads_kv * block_rows;
     if (p.splits > 1 && join_blocks > 0x7fffffffLL / 256) return hipErrorInvalidValue;
-    hipError_t e = fa::launch_kernel(serving_attention_kernel<T, D, kWaves, kPaged>, dim3(static_cast<unsigned>(blocks)),
-                                     dim3(64 * kWaves), stream, a);
+    void (*kernel)(const Args) = nullptr;
+    if constexpr (kWaves <= 2) kernel = serving_few_rows_kernel<T, D, kWaves, kPaged>;
+    else kernel = serving_many_rows_kernel<T, D, kWaves, kPaged>;
+    hipError_t e = fa::launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), stream, a);
     if (e != hipSuccess || p.splits == 1) return e;
     return fa::launch_kernel(serving_join_kernel<T, D, 32 * kWaves, kPaged>, dim3(static_cast<unsigned>(join_blocks)),
                              dim3(256), stream, a, block_rows);
