@@ -362,125 +362,6 @@ __device__ __forceinline__ bool take_block(const Args& a, Block& b, int& split)
     return find_block<R, kPaged>(a, a.slots - 1 - rest / a.splits, head, b) && split < b.splits;
 }
 
-// Few rows (one or two waves of them): bound by the reads of K and V. A step takes
-// one tile, with the copies of the next two in flight.
-template <typename T, int D, int kWaves, bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) void serving_few_rows_kernel(const Args a)
-{
-    using E = Elem<T>;
-    using x8 = typename E::x8;
-    using C = TileCopy<D, kWaves>;
-    constexpr int R = 32 * kWaves;
-    constexpr int kStages = 3;
-    constexpr int kTile = kTileKeys * D;  // elements
-    __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStages * kTile];
-
-    const int lane = threadIdx.x & 63;
-    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
-    const int i = lane & 31;
-    const int h = lane >> 5;
-    Block b;
-    int split;
-    if (!take_block<R, kPaged>(a, b, split)) return;
-    const Rows r = wave_rows<R>(a, b, split, wave, i);
-
-    f32x16 o[D / 32];
-#pragma unroll
-    for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
-    float m = kEmptyBase, l = 0.0f;
-    if (r.t_begin < r.t_end)
-    {
-        const Keys<D, kPaged> keys(a, b);
-        const uint32_t k_row_bytes = static_cast<uint32_t>(a.k_row * 2);
-        const uint32_t v_row_bytes = static_cast<uint32_t>(a.v_row * 2);
-        // A copy's lanes: row and chunk of each lane's 16 bytes, from the half's first row.
-        uint32_t koff[C::kIssues], voff[C::kIssues];
-        {
-            const int sub = (lane % C::kLanes) / C::kChunks;
-            const int pchunk = lane % C::kChunks;
-#pragma unroll
-            for (int u = 0; u < C::kIssues; ++u)
-            {
-                const int row = (u * kWaves + wave) * C::kRows + sub;
-                koff[u] = static_cast<uint32_t>(row & 15) * k_row_bytes + ((pchunk ^ swz_k<D>(row)) * 16);
-                voff[u] = static_cast<uint32_t>(row & 15) * v_row_bytes + ((pchunk ^ swz_v<D>(row)) * 16);
-            }
-        }
-        const uint32_t lds_base = fa::lds_addr(lds);
-        int page_lo = keys.page_of(r.t_begin * kTileKeys), page_hi = keys.page_of(r.t_begin * kTileKeys + 16);
-        auto copy_tile = [&](int t) {
-            const int stage = t % kStages;
-            const auto lo = keys.half_at(t * kTileKeys, page_lo), hi = keys.half_at(t * kTileKeys + 16, page_hi);
-            page_lo = keys.page_of((t + 1) * kTileKeys);
-            page_hi = keys.page_of((t + 1) * kTileKeys + 16);
-#pragma unroll
-            for (int u = 0; u < C::kIssues; ++u)
-            {
-                const bool low = (u * kWaves + wave) * C::kRows < 16;
-                const uint32_t at = lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes;
-                fa::dma16(keys.descriptor(low ? lo.k : hi.k, low ? lo.rows : hi.rows, k_row_bytes), koff[u], at);
-                fa::dma16(keys.descriptor(low ? lo.v : hi.v, low ? lo.rows : hi.rows, v_row_bytes), voff[u],
-                          at + kStages * kTile * 2);
-            }
-        };
-        static_assert(C::kLanes == 64, "whole copies");
-
-        copy_tile(r.t_begin);
-        copy_tile(r.t_begin + 1);
-
-        x8 qr[D / 16];
-        const uint16_t* qp = a.q + q_offset<kPaged>(a, b, r);
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) qr[ks] = *reinterpret_cast<const x8*>(qp + 16 * ks + 8 * h);
-
-        for (int t = r.t_begin; t < r.t_end; ++t)
-        {
-            // Tile t has landed once only tile t+1's copies are in flight; past the
-            // barrier every wave has left tile t-1, whose stage takes tile t+2.
-            fa::wait_vm_lgkm0<2 * C::kIssues>();
-            barrier();
-            copy_tile(t + 2);
-            if (t >= r.t_last) continue;
-            const uint16_t* const stage = lds + (t % kStages) * kTile;
-            f32x16 s = {};
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-                s = E::mfma(*reinterpret_cast<const x8*>(stage + k_read_offset<D>(i, h, ks)), qr[ks], s);
-            if (t >= r.t_mask) mask_tile(s, r.limit - t * kTileKeys - 4 * h);
-            const float m_new = __builtin_elementwise_maximum(m, row_max_raw(s) * a.c_log2 - E::kBias);
-            if (__any(m_new != m))
-            {
-                const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-                l *= alpha;
-#pragma unroll
-                for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
-                m = m_new;
-            }
-            x8 p[2];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-            {
-#pragma clang fp contract(off)
-                // The product is rounded as the base was: the largest score's weight
-                // is exactly 2^kBias however large the score.
-                const float x = s[e] * a.c_log2 - m;
-                p[e >> 3][e & 7] = static_cast<T>(__builtin_amdgcn_exp2f(x));
-            }
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) l = E::add_pair(p[e >> 3][e & 7], p[e >> 3][(e & 7) + 1], l);
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int db = 0; db < D / 32; ++db)
-                    o[db] = E::mfma(read_v<T, D>(stage + kStages * kTile + v_read_offset<D>(lane, db), half), p[half], o[db]);
-        }
-        fa::wait_vm_lgkm0<0>();  // the last copies have landed before the workgroup's LDS goes
-    }
-    store_row<T, D, kPaged>(a, b, r, split, h, o, m, l);
-}
-
 // Keeps a value's producing instructions inside the current block: the compiler
 // cannot sink them past the next branch.
 __device__ __forceinline__ void pin(float& x) { asm volatile("" : "+v"(x)); }
@@ -534,7 +415,7 @@ constexpr float kSumLimit<_Float16> = 32768.0f;
 constexpr float kCoarseBase = 268435456.0f;
 
 template <typename T, int D, int kWaves, bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 8))) void serving_many_rows_kernel(
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 8))) void serving_attention_kernel(
     const Args a)
 {
     using E = Elem<T>;
@@ -611,7 +492,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             copy(half.v, half.rows, v_row_bytes, voff[u],
                  lds_base + (kStages + stage) * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
         };
-        static_assert(kHalves == 1 || (kWaves * C::kRows) % 16 == 0, "every wave's copy u lies in the same half");
+        static_assert(kHalves == 1 || 16 % (kWaves * C::kRows) == 0, "every wave's copy u lies in the same half");
 
         const int t0 = r.t_begin;
         const int cnt = r.t_end - t0;
@@ -832,70 +713,82 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     store_row<T, D, kPaged>(a, b, r, split, h, o, m, l);
 }
 
-// Joins the chunks of one row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c
-// with M the largest base. A workgroup per row; D/4 lanes read a chunk's 4 D
-// bytes, so 256 threads have 1024/D chunks in flight at a time.
-template <typename T, int D, int R, bool kPaged>
-__global__ __launch_bounds__(256) void serving_join_kernel(const Args a, int block_rows)
+// Joins the chunks of a row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c with
+// M the largest base, kept running. D/4 lanes read a chunk's 4 D bytes, so 256
+// threads make 1024/D groups: for few rows with many chunks (kAlone) they all work on
+// one row, chunk by chunk in turn, and meet in LDS; else each takes rows of its own.
+constexpr int kAloneRows = 16;  // rows of a block up to which each has a workgroup to itself
+constexpr int kJoinRows = 32;  // rows of a workgroup that are not kAlone
+
+template <typename T, int D, int R, bool kPaged, bool kAlone>
+__global__ __launch_bounds__(256) void serving_join_kernel(const Args a, int block_parts)
 {
     constexpr int kLanes = D / 4;
-    constexpr int kAtOnce = 256 / kLanes;
-    __shared__ float weight[kMaxSplits];
-    __shared__ f32x4 sums[256];
+    constexpr int kGroups = 256 / kLanes;
     const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.heads_kv));
     const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.heads_kv));
     Block b;
-    if (!find_block<R, kPaged>(a, rest / block_rows, head, b)) return;
-    const int row = b.row0 + rest % block_rows;
-    if (b.splits == 1 || row >= b.rows) return;
-    const int token = row / a.group, qh = row % a.group;
-    const long long pr = part_row<kPaged>(a, b, token, qh) * a.splits;
-
+    if (!find_block<R, kPaged>(a, rest / block_parts, head, b) || b.splits == 1) return;
     const int tid = threadIdx.x;
-    // Every wave finds the base and the sum for itself; wave 0 keeps the weights.
-    float top = kEmptyBase, total = 0.0f;
-    float mv[kMaxSplits / 64], lv[kMaxSplits / 64];
-#pragma unroll
-    for (int x = 0; x < kMaxSplits / 64; ++x)
-    {
-        const int c = 64 * x + (tid & 63);
-        mv[x] = kEmptyBase;
-        lv[x] = 0.0f;
-        if (c < b.splits)
-        {
-            mv[x] = a.base_sum[2 * (pr + c)];
-            lv[x] = a.base_sum[2 * (pr + c) + 1];
-        }
-        top = __builtin_elementwise_maximum(top, mv[x]);
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, off, 64));
-#pragma unroll
-    for (int x = 0; x < kMaxSplits / 64; ++x)
-    {
-        const float w = __builtin_amdgcn_exp2f(mv[x] - top);
-        total += w * lv[x];
-        if (tid < 64) weight[64 * x + tid] = w;
-    }
-    total = fa::wave_sum(total);
-    __syncthreads();
-
-    f32x4 acc = {};
+    const int group = tid / kLanes;
     const int d4 = (tid % kLanes) * 4;
+
+    struct Sum
+    {
+        float top = kEmptyBase, total = 0.0f;
+        f32x4 o = {};
+        __device__ __forceinline__ void add(float m, float l, f32x4 x)
+        {
+            const float t = __builtin_elementwise_maximum(top, m);
+            const float w0 = __builtin_amdgcn_exp2f(top - t), w1 = __builtin_amdgcn_exp2f(m - t);
+            total = total * w0 + l * w1;
+            o = o * w0 + x * w1;
+            top = t;
+        }
+    };
+    auto join = [&](long long pr, int first, int step) {
+        Sum s;
 #pragma unroll 4
-    for (int c = tid / kLanes; c < b.splits; c += kAtOnce)
-        acc += *reinterpret_cast<const f32x4*>(a.part + (pr + c) * D + d4) * weight[c];
-    sums[tid] = acc;
-    __syncthreads();
-    if (tid >= kLanes) return;
+        for (int c = first; c < b.splits; c += step)
+        {
+            const float2 ml = *reinterpret_cast<const float2*>(a.base_sum + 2 * (pr + c));
+            s.add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(a.part + (pr + c) * D + d4));
+        }
+        return s;
+    };
+    auto store = [&](const Sum& s, int token, int qh) {
+        const float inv = s.total > 0.0f ? __builtin_amdgcn_rcpf(s.total) : 0.0f;
+        uint2 w;
+        w.x = pack_pair<T>(s.o[0] * inv, s.o[1] * inv);
+        w.y = pack_pair<T>(s.o[2] * inv, s.o[3] * inv);
+        *reinterpret_cast<uint2*>(a.o + o_offset<kPaged>(a, b, token, qh) + d4) = w;
+    };
+    if constexpr (kAlone)
+    {
+        __shared__ f32x4 parts[256];
+        __shared__ float2 bases[256];
+        const int row = b.row0 + rest % block_parts;
+        if (row >= b.rows) return;
+        const int token = row / a.group, qh = row % a.group;
+        Sum s = join(part_row<kPaged>(a, b, token, qh) * a.splits, group, kGroups);
+        parts[tid] = s.o;
+        bases[tid] = float2{s.top, s.total};
+        __syncthreads();
+        if (tid >= kLanes) return;
 #pragma unroll
-    for (int x = 1; x < kAtOnce; ++x) acc += sums[x * kLanes + tid];
-    const float inv = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
-    uint16_t* op = a.o + o_offset<kPaged>(a, b, token, qh);
-    uint2 w;
-    w.x = pack_pair<T>(acc[0] * inv, acc[1] * inv);
-    w.y = pack_pair<T>(acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<uint2*>(op + d4) = w;
+        for (int g = 1; g < kGroups; ++g) s.add(bases[g * kLanes + tid].x, bases[g * kLanes + tid].y, parts[g * kLanes + tid]);
+        store(s, token, qh);
+    }
+    else
+    {
+        const int first = b.row0 + rest % block_parts * kJoinRows;
+        const int last = min(min(first + kJoinRows, b.row0 + R), b.rows);
+        for (int row = first + group; row < last; row += kGroups)
+        {
+            const int token = row / a.group, qh = row % a.group;
+            store(join(part_row<kPaged>(a, b, token, qh) * a.splits, 0, 1), token, qh);
+        }
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -917,7 +810,7 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
     max_keys = static_cast<int>(std::min<long long>(max_keys, kMaxKeys));
     const int group = heads / heads_kv;
     const long long rows = static_cast<long long>(std::min<long long>(max_queries, tokens)) * group;
-    p.waves = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    p.waves = rows <= 32 ? 4 : rows <= 64 ? 4 : rows <= 128 ? 4 : 8;
     const int R = 32 * p.waves;
     const long long per_seq = (rows + R - 1) / R;
     p.per_seq = static_cast<int>(per_seq);
@@ -931,7 +824,7 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
     }
     const long long blocks = p.slots * heads_kv;
     const long long cus = fa::device_compute_units();
-    const long long target = cus * (p.waves == 1 ? 6 : p.waves == 2 ? 4 : p.waves == 4 ? 2 : 1);
+    const long long target = cus * (p.waves == 2 ? 4 : p.waves == 4 ? 2 : 1);
     const long long least = 256;  // keys per chunk
     long long splits = std::max<long long>(1, std::min<long long>({target / std::max<long long>(1, blocks),
                                                                    (max_keys + least - 1) / least, kMaxSplits}));
@@ -948,15 +841,16 @@ int launch_typed(const Args& a, const Plan& p, int head_rows, hipStream_t stream
     const long long blocks = p.slots * a.heads_kv * p.splits;
     if (blocks > 0x7fffffffLL / (64 * kWaves)) return hipErrorInvalidValue;
     const int block_rows = std::min(32 * kWaves, head_rows);
-    const long long join_blocks = p.slots * a.heads_kv * block_rows;
+    const bool alone = block_rows <= kAloneRows;
+    const int parts = alone ? block_rows : (block_rows + kJoinRows - 1) / kJoinRows;
+    const long long join_blocks = p.slots * a.heads_kv * parts;
     if (p.splits > 1 && join_blocks > 0x7fffffffLL / 256) return hipErrorInvalidValue;
-    void (*kernel)(const Args) = nullptr;
-    if constexpr (kWaves <= 2) kernel = serving_few_rows_kernel<T, D, kWaves, kPaged>;
-    else kernel = serving_many_rows_kernel<T, D, kWaves, kPaged>;
-    hipError_t e = fa::launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), stream, a);
+    const hipError_t e = fa::launch_kernel(serving_attention_kernel<T, D, kWaves, kPaged>,
+                                           dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), stream, a);
     if (e != hipSuccess || p.splits == 1) return e;
-    return fa::launch_kernel(serving_join_kernel<T, D, 32 * kWaves, kPaged>, dim3(static_cast<unsigned>(join_blocks)),
-                             dim3(256), stream, a, block_rows);
+    return fa::launch_kernel(alone ? serving_join_kernel<T, D, 32 * kWaves, kPaged, true>
+                                   : serving_join_kernel<T, D, 32 * kWaves, kPaged, false>,
+                             dim3(static_cast<unsigned>(join_blocks)), dim3(256), stream, a, parts);
 }
 
 template <typename T, int D, bool kPaged>
@@ -964,7 +858,6 @@ int launch_waves(const Args& a, const Plan& p, int head_rows, hipStream_t stream
 {
     switch (p.waves)
     {
-        case 1: return launch_typed<T, D, 1, kPaged>(a, p, head_rows, stream);
         case 2: return launch_typed<T, D, 2, kPaged>(a, p, head_rows, stream);
         case 4: return launch_typed<T, D, 4, kPaged>(a, p, head_rows, stream);
         default: return launch_typed<T, D, 8, kPaged>(a, p, head_rows, stream);
