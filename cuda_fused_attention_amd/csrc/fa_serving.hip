@@ -20,7 +20,6 @@
 #include <cmath>
 #include <cstdint>
 
-#include "fa_fused_schedule.hpp"
 #include "fa_paged.hpp"
 #include "fa_serving_core.hpp"
 
@@ -78,6 +77,8 @@ __device__ __forceinline__ int limit_of(const Args& a, const Block& b, int token
     return a.causal ? max(0, min(b.keys, b.shift + token + 1)) : b.keys;
 }
 
+typedef const __attribute__((address_space(4))) int ConstInt;  // read through the scalar cache
+
 // The block of `slot` (of R rows). False: it holds no row.
 template <int R, bool kPaged>
 __device__ __forceinline__ bool find_block(const Args& a, int slot, int head, Block& b)
@@ -86,37 +87,51 @@ __device__ __forceinline__ bool find_block(const Args& a, int slot, int head, Bl
     b.head = head;
     if constexpr (kPaged)
     {
-        auto start_of = [&](int s) { return max(0, min(a.starts[s], a.tokens)); };
+        auto clamped = [&](int start) { return max(0, min(start, a.tokens)); };
+        int start, end, len;
         if (a.per_seq > 0)
         {
             b.seq = slot / a.per_seq;
             rb = slot % a.per_seq;
+            const ConstInt* const starts = (const ConstInt*)(a.starts + b.seq);
+            start = starts[0];
+            end = starts[1];
+            len = *(const ConstInt*)(a.lens + b.seq);
         }
         else
         {
             // Sequence s owns the slots from floor(first row / R) + s on, at least
-            // as many as it has blocks. The first slots of 64 sequences are
-            // compared at a time, each time one 64th of those left.
+            // as many as it has blocks. 64 sequences are compared at a time, each time
+            // one 64th of those left; the last time the lanes hold their ends and
+            // lengths too.
             const int lane = threadIdx.x & 63;
-            int lo = 0, hi = a.seqs;
-            auto first_slot = [&](int s) {
-                return static_cast<int>(static_cast<long long>(start_of(s)) * a.group / R) + s;
-            };
-            while (hi - lo > 1)
+            int lo = 0, hi = a.seqs, first = 0;
+            while (true)
             {
                 const int step = (hi - lo + 63) / 64;
-                const int s = lo + lane * step;
-                const bool below = s < hi && first_slot(s) <= slot;
-                const int count = max(1, __popcll(__ballot(below)));
-                lo += (count - 1) * step;
+                const int s = min(lo + lane * step, hi - 1);
+                start = a.starts[s];
+                end = a.starts[s + 1];
+                len = a.lens[s];
+                first = static_cast<int>(static_cast<long long>(clamped(start)) * a.group / R) + s;
+                const int below = __popcll(__ballot(lo + lane * step < hi && first <= slot));
+                const int at = max(1, below) - 1;
+                if (step == 1)
+                {
+                    b.seq = lo + at;
+                    start = __builtin_amdgcn_readlane(start, at);
+                    end = __builtin_amdgcn_readlane(end, at);
+                    len = __builtin_amdgcn_readlane(len, at);
+                    rb = slot - __builtin_amdgcn_readlane(first, at);
+                    break;
+                }
+                lo += at * step;
                 hi = min(hi, lo + step);
             }
-            b.seq = uniform(lo);
-            rb = slot - uniform(first_slot(b.seq));
         }
-        b.first_token = uniform(start_of(b.seq));
-        tokens = max(0, uniform(start_of(b.seq + 1)) - b.first_token);
-        const int len = max(0, uniform(a.lens[b.seq]));
+        b.first_token = uniform(clamped(start));
+        tokens = max(0, uniform(clamped(end)) - b.first_token);
+        len = max(0, uniform(len));
         b.keys = static_cast<int>(min(static_cast<long long>(len), static_cast<long long>(a.table_width) << a.block_shift));
         b.shift = len - tokens;
         b.rows = min(tokens, a.max_queries) * a.group;
@@ -126,14 +141,17 @@ __device__ __forceinline__ bool find_block(const Args& a, int slot, int head, Bl
         b.seq = slot / a.per_seq;
         rb = slot % a.per_seq;
         b.first_token = 0;
-        b.keys = a.lens ? max(0, min(uniform(a.lens[b.seq]), a.max_keys)) : a.max_keys;
+        b.keys = a.lens ? max(0, min(*(const ConstInt*)(a.lens + b.seq), a.max_keys)) : a.max_keys;
         b.shift = 0;
         b.rows = a.max_queries * a.group;
     }
     if (rb < 0 || static_cast<long long>(rb) * R >= b.rows) return false;
-    b.row0 = rb * R;
-    b.end = limit_of(a, b, (min(b.row0 + R, b.rows) - 1) / a.group);
-    b.splits = max(1, min(a.splits, (b.end + a.chunk - 1) / a.chunk));
+    b.seq = uniform(b.seq);
+    b.keys = uniform(b.keys);
+    b.rows = uniform(b.rows);
+    b.row0 = uniform(rb * R);
+    b.end = uniform(limit_of(a, b, (min(b.row0 + R, b.rows) - 1) / a.group));
+    b.splits = uniform(max(1, min(a.splits, (b.end + a.chunk - 1) / a.chunk)));
     return true;
 }
 
@@ -152,19 +170,19 @@ __device__ __forceinline__ long long part_row(const Args& a, const Block& b, int
 template <int D, bool kPaged>
 struct Keys
 {
-    typedef const __attribute__((address_space(4))) int ConstInt;
-
-    // Sixteen keys: byte addresses of the first and the rows of them that exist;
-    // the others of a copy read as zero, and so does a page outside the cache.
+    // Sixteen keys: byte addresses of the first, and the bytes from it on that hold
+    // keys. What a copy asks for past those reads as zero: keys past the end, and a
+    // page outside the cache.
     struct Half
     {
         uint64_t k, v;
-        int rows;
+        uint32_t k_bytes, v_bytes;
     };
 
     const Args& a;
     uint64_t k_base, v_base;
     uint64_t table;
+    uint32_t k_row_bytes, v_row_bytes;
     int end;
 
     __device__ __forceinline__ Keys(const Args& args, const Block& b) : a(args), end(b.end)
@@ -179,6 +197,8 @@ struct Keys
         k_base = uniform(k_base);
         v_base = uniform(v_base);
         table = uniform(reinterpret_cast<uint64_t>(a.table) + static_cast<uint64_t>(b.seq * a.table_stride * 4));
+        k_row_bytes = uniform(static_cast<uint32_t>(a.k_row * 2));
+        v_row_bytes = uniform(static_cast<uint32_t>(a.v_row * 2));
     }
 
     // The page that holds `key` (the last one of the row for a key past it).
@@ -187,43 +207,53 @@ struct Keys
     {
         if constexpr (!kPaged) return 0;
         const unsigned entry = static_cast<unsigned>(min(key >> a.block_shift, a.table_width - 1));
-        return *reinterpret_cast<ConstInt*>(table + static_cast<uint64_t>(entry) * 4);
+        return *(const ConstInt*)(table + static_cast<uint64_t>(entry) * 4);
     }
 
+    // Pages are at most 2^34 elements apart and a page's rows within 2^30, in steps
+    // of 16 bytes (host-side checks): 32-bit products but for the page's.
     __device__ __forceinline__ Half half_at(int key, int page) const
     {
         Half r;
-        r.rows = max(0, min(16, end - key));
+        const int left = end - key;
+        auto bytes = [&](uint32_t row_bytes) {
+            return left >= 16 ? 16 * row_bytes : static_cast<uint32_t>(max(left, 0)) * row_bytes;
+        };
         if constexpr (kPaged)
         {
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.num_blocks)) r.rows = page = 0;
-            const int in_page = key & ((1 << a.block_shift) - 1);
-            const uint64_t off = (static_cast<uint64_t>(page) * static_cast<uint64_t>(a.k_seq) +
-                                  static_cast<uint64_t>(in_page) * static_cast<uint64_t>(a.k_row)) * 2;
+            const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
+            const uint32_t at = there ? static_cast<uint32_t>(page) : 0u;
+            const uint32_t in_page = static_cast<uint32_t>(key) & ((1u << a.block_shift) - 1);
+            const uint64_t off = ((static_cast<uint64_t>(at) * static_cast<uint32_t>(a.k_seq >> 3)) << 4) +
+                                 in_page * k_row_bytes;
             r.k = k_base + off;
             r.v = v_base + off;
+            r.k_bytes = r.v_bytes = there ? bytes(k_row_bytes) : 0u;
         }
         else
         {
-            r.k = k_base + static_cast<uint64_t>(key) * static_cast<uint64_t>(a.k_row * 2);
-            r.v = v_base + static_cast<uint64_t>(key) * static_cast<uint64_t>(a.v_row * 2);
+            r.k = k_base + static_cast<uint64_t>(static_cast<uint32_t>(key)) * k_row_bytes;
+            r.v = v_base + static_cast<uint64_t>(static_cast<uint32_t>(key)) * v_row_bytes;
+            r.k_bytes = bytes(k_row_bytes);
+            r.v_bytes = bytes(v_row_bytes);
         }
         return r;
     }
 
-    static __device__ __forceinline__ i32x4 descriptor(uint64_t base, int rows, uint32_t row_bytes)
+    // Buffer descriptor of `bytes` bytes from `base` on (48-bit addresses, stride 0).
+    static __device__ __forceinline__ i32x4 descriptor(uint64_t base, uint32_t bytes)
     {
         i32x4 r;
         r[0] = uniform(static_cast<int>(static_cast<uint32_t>(base)));
         r[1] = uniform(static_cast<int>(static_cast<uint32_t>(base >> 32) & 0xffffu));
-        r[2] = uniform(rows > 0 ? static_cast<int>((rows - 1) * row_bytes + D * 2) : 0);
+        r[2] = uniform(static_cast<int>(bytes));
         r[3] = static_cast<int>(fa::kRawBufferConfig);
         return r;
     }
 
-    // Element offset of a lane's key below `end`, for the rare paths that read
-    // keys outside the pipeline; false: it holds zeros.
-    __device__ __forceinline__ bool lane_key(int key, uint64_t& k, uint64_t& v) const
+    // Address of a lane's key, for the rare path that reads keys outside the
+    // pipeline; false: it holds zeros.
+    __device__ __forceinline__ bool lane_key(int key, uint64_t& k) const
     {
         bool there = key < end;
         int page = 0;
@@ -232,9 +262,7 @@ struct Keys
             if (there) page = *reinterpret_cast<const int*>(table + static_cast<uint64_t>(key >> a.block_shift) * 4);
             there = there && static_cast<unsigned>(page) < static_cast<unsigned>(a.num_blocks);
         }
-        const Half r = half_at(key, there ? page : 0);
-        k = r.k;
-        v = r.v;
+        k = half_at(key, there ? page : 0).k;
         return there;
     }
 };
@@ -265,8 +293,8 @@ __device__ __forceinline__ Rows wave_rows(const Args& a, const Block& b, int spl
     r.t_end = (k_end + kTileKeys - 1) / kTileKeys;
     const int first = b.row0 + 32 * wave;
     const int wave_end = first < b.rows ? limit_of(a, b, min(first + 31, b.rows - 1) / a.group) : 0;
-    r.t_last = min(r.t_end, (wave_end + kTileKeys - 1) / kTileKeys);
-    r.t_mask = limit_of(a, b, min(first, b.rows - 1) / a.group) / kTileKeys;
+    r.t_last = uniform(min(r.t_end, (wave_end + kTileKeys - 1) / kTileKeys));
+    r.t_mask = uniform(limit_of(a, b, min(first, b.rows - 1) / a.group) / kTileKeys);
     return r;
 }
 
@@ -357,9 +385,10 @@ __device__ __forceinline__ bool take_block(const Args& a, Block& b, int& split)
 {
     const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.heads_kv));
     const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.heads_kv));
-    split = rest % a.splits;
-    // Late rows see the most keys: they start first.
-    return find_block<R, kPaged>(a, a.slots - 1 - rest / a.splits, head, b) && split < b.splits;
+    // Late rows see the most keys: they start first. First chunks, which every block
+    // has, before second ones: the slots alternate over the XCDs that a head has.
+    split = rest / a.slots;
+    return find_block<R, kPaged>(a, a.slots - 1 - rest % a.slots, head, b) && split < b.splits;
 }
 
 // Keeps a value's producing instructions inside the current block: the compiler
@@ -397,6 +426,43 @@ __device__ __forceinline__ void weigh(const f32x16& s, int first, typename Elem<
     for (int e = 0; e < 8; e += 2) sum = Elem<T>::add_pair(p[e], p[e + 1], sum);
 }
 
+// step(masked, P, jj) for jj = 0 .. count-1 with P = jj modulo 6, a multiple of the
+// stages and of the two score buffers, as a compile-time constant. Whole rounds in
+// which no step's next tile is masked (jj < plain) take steps without the mask: where
+// it is a branch, the compiler keeps the masked scores apart and copies all 16 on the
+// path that masks nothing (a 2048 x 32768 chunk: 999 -> 908 us together with scalar
+// copy addresses). Written out step by step: a recursive template keeps more
+// registers live.
+template <class Step>
+__device__ __forceinline__ void walk(int count, int plain, Step&& step)
+{
+    int jj = 0;
+    for (const int whole = min(count, plain) / 6 * 6; jj < whole; jj += 6)
+    {
+        step(std::false_type{}, std::integral_constant<int, 0>{}, jj);
+        step(std::false_type{}, std::integral_constant<int, 1>{}, jj + 1);
+        step(std::false_type{}, std::integral_constant<int, 2>{}, jj + 2);
+        step(std::false_type{}, std::integral_constant<int, 3>{}, jj + 3);
+        step(std::false_type{}, std::integral_constant<int, 4>{}, jj + 4);
+        step(std::false_type{}, std::integral_constant<int, 5>{}, jj + 5);
+    }
+    while (jj < count)
+    {
+        step(std::true_type{}, std::integral_constant<int, 0>{}, jj);
+        if (++jj >= count) break;
+        step(std::true_type{}, std::integral_constant<int, 1>{}, jj);
+        if (++jj >= count) break;
+        step(std::true_type{}, std::integral_constant<int, 2>{}, jj);
+        if (++jj >= count) break;
+        step(std::true_type{}, std::integral_constant<int, 3>{}, jj);
+        if (++jj >= count) break;
+        step(std::true_type{}, std::integral_constant<int, 4>{}, jj);
+        if (++jj >= count) break;
+        step(std::true_type{}, std::integral_constant<int, 5>{}, jj);
+        ++jj;
+    }
+}
+
 // Many rows (128 or 256 of a key head): bound by the matrix cores, beside which
 // the exponentials have to hide. The step of the fused self-attention kernel: in
 // block A the matrix cores compute tile j+1's scores while the vector unit ends
@@ -415,15 +481,15 @@ constexpr float kSumLimit<_Float16> = 32768.0f;
 constexpr float kCoarseBase = 268435456.0f;
 
 template <typename T, int D, int kWaves, bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 8))) void serving_attention_kernel(
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWaves > 2 ? 2 : 1, 8))) void serving_attention_kernel(
     const Args a)
 {
     using E = Elem<T>;
     using x8 = typename E::x8;
     using C = TileCopy<D, kWaves>;
     constexpr int R = 32 * kWaves;
-    constexpr int kStages = fa::kFusedStages;
-    static_assert(kStages == 3, "the step's copies run three K and two V tiles ahead");
+    constexpr int kStages = 3;  // per tensor; four measured no faster
+    static_assert(6 % kStages == 0, "the walk's rounds");
     constexpr int kTile = kTileKeys * D;  // elements
     constexpr int kI = C::kIssues;
     // A wave's copies of a tile lie in one half of it, or in both.
@@ -447,9 +513,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
     {
         const Keys<D, kPaged> keys(a, b);
         const float c_log2 = a.c_log2;
-        const uint32_t k_row_bytes = static_cast<uint32_t>(a.k_row * 2);
-        const uint32_t v_row_bytes = static_cast<uint32_t>(a.v_row * 2);
-        uint32_t koff[kI], voff[kI];
+        uint32_t koff[kI], voff[kI];  // a copy's lanes: row and chunk from the half's first row
+
         {
             const int sub = (lane % C::kLanes) / C::kChunks;
             const int pchunk = lane % C::kChunks;
@@ -457,8 +522,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             for (int u = 0; u < kI; ++u)
             {
                 const int row = (u * kWaves + wave) * C::kRows + sub;
-                koff[u] = static_cast<uint32_t>(row & 15) * k_row_bytes + ((pchunk ^ swz_k<D>(row)) * 16);
-                voff[u] = static_cast<uint32_t>(row & 15) * v_row_bytes + ((pchunk ^ swz_v<D>(row)) * 16);
+                koff[u] = static_cast<uint32_t>(row & 15) * keys.k_row_bytes + ((pchunk ^ swz_k<D>(row)) * 16);
+                voff[u] = static_cast<uint32_t>(row & 15) * keys.v_row_bytes + ((pchunk ^ swz_v<D>(row)) * 16);
             }
         }
         const uint32_t lds_base = fa::lds_addr(lds);
@@ -478,18 +543,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             for (int x = 0; x < kHalves; ++x) p.half[x] = keys.half_at(t * kTileKeys + half0 + 16 * x, pages[x]);
             return p;
         };
-        auto copy = [&](uint64_t base, int rows, uint32_t row_bytes, uint32_t off, uint32_t at) {
-            const i32x4 d = keys.descriptor(base, rows, row_bytes);
+        auto copy = [&](i32x4 d, uint32_t off, uint32_t at) {
             if constexpr (C::kLanes == 64) fa::dma16(d, off, at);
             else if (lane < C::kLanes) fa::dma16(d, off, at);
         };
         auto copy_k = [&](const Place& p, int stage, int u) {
             const auto& half = p.half[kHalves == 1 ? 0 : (u * kWaves * C::kRows) >> 4];
-            copy(half.k, half.rows, k_row_bytes, koff[u], lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
+            copy(keys.descriptor(half.k, half.k_bytes), koff[u],
+                 lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
         };
         auto copy_v = [&](const Place& p, int stage, int u) {
             const auto& half = p.half[kHalves == 1 ? 0 : (u * kWaves * C::kRows) >> 4];
-            copy(half.v, half.rows, v_row_bytes, voff[u],
+            copy(keys.descriptor(half.v, half.v_bytes), voff[u],
                  lds_base + (kStages + stage) * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
         };
         static_assert(kHalves == 1 || 16 % (kWaves * C::kRows) == 0, "every wave's copy u lies in the same half");
@@ -499,24 +564,28 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
         const int lw = r.t_last - t0 - 1;             // last step this wave computes
         const int j_mask = min(lw, r.t_mask - t0 - 1);  // first step whose next tile is masked
 
-        // Prologue: K 0..2 and V 0..1; `ahead` is the place of tile 3 (K next, V a step
-        // later), `behind` that of tile 2 (V next).
+        // Prologue: K 0, then K x + 1 and V x in the order of their use. `ahead` is the
+        // place of tile kStages (K next, V a step later), `behind` that of the tile
+        // before it (V next).
         Place ahead, behind;
         fetch_pages(t0);
+        behind = place_of(t0);
+        fetch_pages(t0 + 1);
 #pragma unroll
-        for (int x = 0; x < kStages; ++x)
+        for (int u = 0; u < kI; ++u) copy_k(behind, 0, u);
+#pragma unroll
+        for (int x = 1; x < kStages; ++x)
         {
-            const Place p = place_of(t0 + x);
+            ahead = place_of(t0 + x);
             fetch_pages(t0 + x + 1);
 #pragma unroll
-            for (int u = 0; u < kI; ++u) copy_k(p, x, u);
-            if (x < 2)
+            for (int u = 0; u < kI; ++u) copy_k(ahead, x, u);
 #pragma unroll
-                for (int u = 0; u < kI; ++u) copy_v(p, x, u);
-            else behind = p;
+            for (int u = 0; u < kI; ++u) copy_v(behind, x - 1, u);
+            behind = ahead;
         }
-        ahead = place_of(t0 + 3);
-        fetch_pages(t0 + 4);
+        ahead = place_of(t0 + kStages);
+        fetch_pages(t0 + kStages + 1);
 
         x8 qr[D / 16];
         const uint16_t* qp = a.q + q_offset<kPaged>(a, b, r);
@@ -556,8 +625,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             if (__any(base != kEmptyBase && __builtin_fabsf(base) >= kCoarseBase)) limit_bits = __builtin_bit_cast(int, -1.0f);
             limit_bits = uniform(limit_bits);
         };
-        // The first K tile: everything but K 1, K 2 and V 0, V 1 has landed.
-        fa::wait_vm_lgkm0<4 * kI>();
+        // K 0 has landed: kStages - 1 tiles of K and of V may fly.
+        fa::wait_vm_lgkm0<2 * (kStages - 1) * kI>();
         barrier();
         if (lw >= 0)
         {
@@ -570,19 +639,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             weigh<T, false>(sbuf[0], 0, p_lo[0], m, c_log2, tsum);
             note_base(m);
         }
-        fa::wait_vm_lgkm0<0>();
-        barrier();  // every prologue tile has landed; K 0's stage is free
+        // K 1 and V 0 have landed, K 0's stage is free.
+        fa::wait_vm_lgkm0<(2 * kStages - 4) * kI>();
+        barrier();
         load_k(1, 0, D / 16);
 
         // The base lags (see above): tile jj's P was zeroed; its scores again, the base
         // at the row maximum, O and l rescaled, its P V from V's stage (intact until the
         // next step's copies), and the first half of the next tile's exponentials again.
-        auto rebase = [&](auto par_tag, int jj) {
+        auto rebase = [&](auto par_tag, int jj) __attribute__((always_inline)) {
             constexpr int P = decltype(par_tag)::value;
             constexpr int B = P & 1;
             const int t = t0 + jj;
-            uint64_t kp, vp;
-            const bool there = keys.lane_key(t * kTileKeys + i, kp, vp);
+            uint64_t kp;
+            const bool there = keys.lane_key(t * kTileKeys + i, kp);
             f32x16 st = {};
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
@@ -635,7 +705,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
 #pragma unroll
             for (int ks = first; ks < first + count; ++ks) s = E::mfma(ka[ks], qr[ks], s);
         };
-        auto step = [&](auto par_tag, int jj) {
+        auto step = [&](auto masked_tag, auto par_tag, int jj) __attribute__((always_inline)) {
             constexpr int P = decltype(par_tag)::value;
             constexpr int B = P & 1;
             // Block A
@@ -654,8 +724,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             }
             pin8(p_hi);
             pin(tsum);
-            // K jj+2 and V jj+1 have landed (K jj+3 may fly), every LDS read is done.
-            fa::wait_vm_lgkm0<kI>();
+            // K jj+2 and V jj+1 have landed (what was issued after them may fly), every
+            // LDS read is done.
+            fa::wait_vm_lgkm0<(2 * kStages - 5) * kI>();
             barrier();
             // Block B
             const bool rare = __any(tsum > __builtin_bit_cast(float, limit_bits));
@@ -668,7 +739,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             }
             l += tsum;
             // Past the wave's last tile the next scores are of a stage that nobody needs.
-            if (jj >= j_mask) mask_tile(sbuf[B ^ 1], jj == lw ? -kTileKeys : r.limit - (t0 + jj + 1) * kTileKeys - 4 * h);
+            if constexpr (decltype(masked_tag)::value) mask_tile(sbuf[B ^ 1], jj == lw ? -kTileKeys : r.limit - (t0 + jj + 1) * kTileKeys - 4 * h);
             __builtin_amdgcn_sched_barrier(0);
             const x8 p_cur[2] = {p_lo[B], p_hi};
             tsum = 0.0f;
@@ -677,7 +748,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
             {
                 pv_part(p_cur, c * kMfmaPer, 1);
                 __builtin_amdgcn_sched_barrier(0);
-                copy_v(behind, (P + 2) % kStages, c);
+                copy_v(behind, (P + kStages - 1) % kStages, c);
                 __builtin_amdgcn_sched_barrier(0);
                 load_k((P + 2) % kStages, c * kKPer, kKPer);
                 pv_part(p_cur, c * kMfmaPer + 1, kMfmaPer - 1);
@@ -685,28 +756,28 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2, 
                 __builtin_amdgcn_sched_barrier(0);
             }
             behind = ahead;
-            ahead = place_of(t0 + jj + 4);
-            fetch_pages(t0 + jj + 5);
+            ahead = place_of(t0 + jj + kStages + 1);
+            fetch_pages(t0 + jj + kStages + 2);
             pin8(p_lo[B ^ 1]);
             pin(tsum);
             if (rare) rebase(par_tag, jj);
             pin(l);
         };
         const int active = max(0, min(cnt, lw + 1));
-        fa::fused_group_walk(active, step);
+        walk(active, max(0, j_mask), step);
         // The steps past this wave's last tile: its share of the copies and the barriers.
         for (int jj = active; jj < cnt; ++jj)
         {
             const int stage = jj % kStages;
 #pragma unroll
             for (int u = 0; u < kI; ++u) copy_k(ahead, stage, u);
-            fa::wait_vm_lgkm0<kI>();
+            fa::wait_vm_lgkm0<(2 * kStages - 5) * kI>();
             barrier();
 #pragma unroll
-            for (int u = 0; u < kI; ++u) copy_v(behind, (stage + 2) % kStages, u);
+            for (int u = 0; u < kI; ++u) copy_v(behind, (stage + kStages - 1) % kStages, u);
             behind = ahead;
-            ahead = place_of(t0 + jj + 4);
-            fetch_pages(t0 + jj + 5);
+            ahead = place_of(t0 + jj + kStages + 1);
+            fetch_pages(t0 + jj + kStages + 2);
         }
         fa::wait_vm_lgkm0<0>();  // the last copies have landed before the workgroup's LDS goes
     }
