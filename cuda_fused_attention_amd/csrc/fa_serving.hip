@@ -338,18 +338,23 @@ __device__ __forceinline__ typename Elem<T>::x8 read_v(const uint16_t* base, int
     return __builtin_bit_cast(typename Elem<T>::x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// The lane's row of O: normalised to the element type, or the partial result of
-// one chunk.
+// A wave's rows of O: the partial result of one chunk in 32 bits, or normalised to
+// the element type. A lane holds pieces of 4 dims of its row. In 32 bits they are
+// stored as they are. The 8-byte pieces of the whole rows would touch 32 rows at a
+// time (2.1-2.5 us at the end of every workgroup of many rows): 128 bytes of each row
+// at a time go through `buf` (4 KiB of LDS of the wave's own, 16-byte pieces swizzled
+// by row) and leave as whole lines.
 template <typename T, int D, bool kPaged>
-__device__ __forceinline__ void store_row(const Args& a, const Block& b, const Rows& r, int split, int h,
-                                          const f32x16 (&o)[D / 32], float m, float l)
+__device__ __forceinline__ void store_rows(const Args& a, const Block& b, const Rows& r, int split, int lane,
+                                           const f32x16 (&o)[D / 32], float m, float l, uint4* buf)
 {
+    const int i = lane & 31, h = lane >> 5;
     float la, lb;
     row_halves(l, la, lb);
     l = la + lb;
-    if (r.row >= b.rows) return;
     if (b.splits > 1)
     {
+        if (r.row >= b.rows) return;
         const long long pr = part_row<kPaged>(a, b, r.token, r.qh) * a.splits + split;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
@@ -357,26 +362,40 @@ __device__ __forceinline__ void store_row(const Args& a, const Block& b, const R
             for (int g = 0; g < 4; ++g)
                 *reinterpret_cast<f32x4*>(a.part + pr * D + 32 * db + 8 * g + 4 * h) =
                     f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-        if (h == 0)
-        {
-            a.base_sum[2 * pr] = m;
-            a.base_sum[2 * pr + 1] = l;
-        }
+        if (h == 0) *reinterpret_cast<float2*>(a.base_sum + 2 * pr) = float2{m, l};
         return;
     }
     // A row that saw nothing has the sum 0 and gives 0; a NaN sum leaves O's NaN.
     const float inv = l > 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f;
-    uint16_t* op = a.o + o_offset<kPaged>(a, b, r.token, r.qh);
+    // As they leave, lane / 8 of every 8 rows and 16 bytes of its 128: the place of
+    // that row comes from the lane that holds it (-1: no row).
+    const long long mine = r.row < b.rows ? o_offset<kPaged>(a, b, r.token, r.qh) : -1;
+    const int piece = lane & 7;
+    long long at[4];
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+    for (int u = 0; u < 4; ++u) at[u] = __shfl(mine, 8 * u + (lane >> 3), 64);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+    for (int half = 0; half < D / 64; ++half)
+    {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
         {
+            const f32x16& ob = o[2 * half + x / 4];
             uint2 w;
-            w.x = pack_pair<T>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv);
-            w.y = pack_pair<T>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv);
-            *reinterpret_cast<uint2*>(op + 32 * db + 8 * g + 4 * h) = w;
+            w.x = pack_pair<T>(ob[4 * (x % 4)] * inv, ob[4 * (x % 4) + 1] * inv);
+            w.y = pack_pair<T>(ob[4 * (x % 4) + 2] * inv, ob[4 * (x % 4) + 3] * inv);
+            reinterpret_cast<uint2*>(buf + i * 8 + (x ^ (i & 7)))[h] = w;
         }
+        fa::wait_vm_lgkm0<63>();  // the wave's own writes; nobody else touches `buf`
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+        {
+            const int row = 8 * u + (lane >> 3);
+            const uint4 x = buf[row * 8 + (piece ^ (row & 7))];
+            if (at[u] >= 0) *reinterpret_cast<uint4*>(a.o + at[u] + 64 * half + 8 * piece) = x;
+        }
+        fa::wait_vm_lgkm0<63>();
+    }
 }
 
 // The block and the chunk of this workgroup; false: nothing to do.
@@ -494,7 +513,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
     constexpr int kI = C::kIssues;
     // A wave's copies of a tile lie in one half of it, or in both.
     constexpr int kHalves = kI > 1 ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStages * kTile];
+    constexpr int kStoreElems = kWaves * 2048;  // 4 KiB a wave at the end (store_rows)
+    constexpr int kLdsElems = 2 * kStages * kTile > kStoreElems ? 2 * kStages * kTile : kStoreElems;
+    __shared__ __attribute__((aligned(16))) uint16_t lds[kLdsElems];
 
     const int lane = threadIdx.x & 63;
     const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
@@ -779,9 +800,12 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
             ahead = place_of(t0 + jj + kStages + 1);
             fetch_pages(t0 + jj + kStages + 2);
         }
-        fa::wait_vm_lgkm0<0>();  // the last copies have landed before the workgroup's LDS goes
+        // Every copy has landed and every wave has read its last tile: the stages are free.
+        fa::wait_vm_lgkm0<0>();
+        barrier();
     }
-    store_row<T, D, kPaged>(a, b, r, split, h, o, m, l);
+    if (b.row0 + 32 * wave < b.rows)
+        store_rows<T, D, kPaged>(a, b, r, split, lane, o, m, l, reinterpret_cast<uint4*>(lds) + wave * 256);
 }
 
 // Joins the chunks of a row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c with
@@ -817,13 +841,40 @@ __global__ __launch_bounds__(256) void serving_join_kernel(const Args a, int blo
             top = t;
         }
     };
+    // kBatch chunks' values are under way together.
     auto join = [&](long long pr, int first, int step) {
+        constexpr int kBatch = 8;
         Sum s;
-#pragma unroll 4
-        for (int c = first; c < b.splits; c += step)
+        for (int c0 = first; c0 < b.splits; c0 += kBatch * step)
         {
-            const float2 ml = *reinterpret_cast<const float2*>(a.base_sum + 2 * (pr + c));
-            s.add(ml.x, ml.y, *reinterpret_cast<const f32x4*>(a.part + (pr + c) * D + d4));
+            float2 ml[kBatch];
+            f32x4 x[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+            {
+                const int c = c0 + u * step;
+                ml[u] = float2{kEmptyBase, 0.0f};
+                x[u] = f32x4{};
+                if (c < b.splits)
+                {
+                    ml[u] = *reinterpret_cast<const float2*>(a.base_sum + 2 * (pr + c));
+                    x[u] = *reinterpret_cast<const f32x4*>(a.part + (pr + c) * D + d4);
+                }
+            }
+            float top = s.top;
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) top = __builtin_elementwise_maximum(top, ml[u].x);
+            const float w = __builtin_amdgcn_exp2f(s.top - top);
+            s.total *= w;
+            s.o *= w;
+            s.top = top;
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+            {
+                const float wu = __builtin_amdgcn_exp2f(ml[u].x - top);
+                s.total += ml[u].y * wu;
+                s.o += x[u] * wu;
+            }
         }
         return s;
     };

@@ -14,7 +14,7 @@ run on the current stream of the tensors' device. Forward only.
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple, Optional
+from typing import Optional
 
 import cuda_fused_attention_amd as _fa
 
@@ -39,13 +39,28 @@ class PagedCache:
         self.num_blocks, self.heads_kv, self.block_size, self.head_dim = k.shape
 
 
-class PagedSlots(NamedTuple):
-    """What paged_slots writes beside the block table."""
+class PagedSlots:
+    """What paged_slots writes beside the block table: query_starts int32
+    [num_seqs + 1], kv_lens int32 [num_seqs], slot_map int64 [max_tokens] and
+    blocks_taken int32 [1], contiguous on one device. Checked when it is made."""
 
-    query_starts: object  # int32 [num_seqs + 1]
-    kv_lens: object       # int32 [num_seqs]
-    slot_map: object      # int64 [max_tokens]
-    blocks_taken: object  # int32 [1]
+    __slots__ = ("query_starts", "kv_lens", "slot_map", "blocks_taken", "num_seqs", "max_tokens", "device")
+
+    def __init__(self, query_starts, kv_lens, slot_map, blocks_taken):
+        torch = _torch or _bind()
+        device, num_seqs, max_tokens = kv_lens.device, kv_lens.numel(), slot_map.numel()
+        for x, n, dtype, name in ((query_starts, num_seqs + 1, torch.int32, "query_starts"),
+                                  (kv_lens, num_seqs, torch.int32, "kv_lens"),
+                                  (slot_map, max_tokens, torch.int64, "slot_map"),
+                                  (blocks_taken, 1, torch.int32, "blocks_taken")):
+            _vector(x, n, device, dtype, name)
+        for name, value in (("query_starts", query_starts), ("kv_lens", kv_lens), ("slot_map", slot_map),
+                            ("blocks_taken", blocks_taken), ("num_seqs", num_seqs), ("max_tokens", max_tokens),
+                            ("device", device)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("PagedSlots cannot be changed")
 
 
 # ---------------------------------------------------------------- C entry points
@@ -158,15 +173,17 @@ def _need(ok: bool, what: str):
 
 def _vector(x, n: int, device, dtype, name: str):
     """`x` is a contiguous vector of n integers on this device."""
-    if x.dtype != dtype or x.device != device or tuple(x.shape) != (n,) or not x.is_contiguous():
+    if x.dtype is not dtype or x.dim() != 1 or x.numel() != n or not x.is_contiguous() or x.device != device:
         raise ValueError(f"{name} must be a contiguous {dtype} tensor [{n}] on {device}")
 
 
 def _table(table, num_seqs: int, device):
     """(width, row stride) of a block table."""
-    if table.dtype != _torch.int32 or table.device != device or table.dim() != 2 or table.shape[0] != num_seqs:
+    if table.dtype is not _torch.int32 or table.dim() != 2 or table.device != device:
         raise ValueError(f"block_table must be an int32 tensor [{num_seqs}, width] on {device}")
-    width = table.shape[1]
+    rows, width = table.shape
+    if rows != num_seqs:
+        raise ValueError(f"block_table has {rows} rows for {num_seqs} sequences")
     stride, column = table.stride()
     if num_seqs < 2:
         stride = max(width, 1)
@@ -189,14 +206,14 @@ def _strides_of(x, name: str):
 
 
 def _like_q(out, q):
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+    if out.dtype is not q.dtype or out.shape != q.shape or out.device != q.device:
         raise ValueError("out must have q's shape, type and device")
 
 
 def _workspace_room(workspace, device) -> int:
     if workspace.device != device or not workspace.is_contiguous():
         raise ValueError(f"workspace must be a contiguous tensor on {device}")
-    return workspace.numel() * workspace.element_size()
+    return workspace.nbytes
 
 
 def _too_small(workspace, have: int, nbytes: int):
@@ -248,18 +265,15 @@ def paged_slots(cached_lens, new_lens, block_table, free_blocks, block_size: int
     num_seqs, num_free = cached_lens.numel(), free_blocks.numel()
     if out is None:
         out = paged_slots_buffers(num_seqs, max_tokens, device)
-    starts, kv_lens, slot_map, taken = out
+    elif out.num_seqs != num_seqs or out.max_tokens != max_tokens or out.device != device:
+        raise ValueError(f"out is for {out.num_seqs} sequences and {out.max_tokens} tokens on {out.device}")
     int32 = torch.int32
     _vector(cached_lens, num_seqs, device, int32, "cached_lens")
     _vector(new_lens, num_seqs, device, int32, "new_lens")
     _vector(free_blocks, num_free, device, int32, "free_blocks")
-    _vector(starts, num_seqs + 1, device, int32, "query_starts")
-    _vector(kv_lens, num_seqs, device, int32, "kv_lens")
-    _vector(slot_map, max_tokens, device, torch.int64, "slot_map")
-    _vector(taken, 1, device, int32, "blocks_taken")
     width, stride = _table(block_table, num_seqs, device)
-    launch_paged_slots(cached_lens, new_lens, block_table, free_blocks, starts, kv_lens, slot_map, taken, num_seqs, width,
-                       stride, num_free, block_size, max_tokens)
+    launch_paged_slots(cached_lens, new_lens, block_table, free_blocks, out.query_starts, out.kv_lens, out.slot_map,
+                       out.blocks_taken, num_seqs, width, stride, num_free, block_size, max_tokens)
     return out
 
 
@@ -273,9 +287,10 @@ def paged_append(k, v, slot_map, cache: PagedCache) -> None:
     tokens = slot_map.numel()
     _vector(slot_map, tokens, device, _torch.int64, "slot_map")
     shape = (tokens, cache.heads_kv, cache.head_dim)
-    for x in (k, v):
-        if tuple(x.shape) != shape or x.dtype != cache.dtype or x.device != device:
-            raise ValueError(f"k and v must be {cache.dtype} tensors {list(shape)} on {device}")
+    dtype = cache.dtype
+    if (k.dtype is not dtype or v.dtype is not dtype or k.shape != shape or v.shape != shape or k.device != device
+            or v.device != device):
+        raise ValueError(f"k and v must be {dtype} tensors {list(shape)} on {device}")
     launch_paged_append(k, v, slot_map, cache, tokens, _strides_of(k, "k"), _strides_of(v, "v"))
 
 
@@ -303,9 +318,11 @@ def attention_paged(q, cache: PagedCache, block_table, query_starts, kv_lens, ma
         with _torch.cuda.device(device):
             return attention_paged(q, cache, block_table, query_starts, kv_lens, max_query_len, max_kv_len, causal, out,
                                    workspace)
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.dtype != cache.dtype or q.device != device:
+    if q.dim() != 3 or q.dtype is not cache.dtype or q.device != device:
         raise ValueError(f"q must be a {cache.dtype} tensor [tokens, heads, {cache.head_dim}] on {device}")
     tokens, heads, head_dim = q.shape
+    if head_dim != cache.head_dim:
+        raise ValueError(f"q has head_dim {head_dim}, the cache {cache.head_dim}")
     num_seqs = kv_lens.numel()
     _vector(kv_lens, num_seqs, device, _torch.int32, "kv_lens")
     _vector(query_starts, num_seqs + 1, device, _torch.int32, "query_starts")
