@@ -925,36 +925,112 @@ struct Plan
     size_t workspace;
 };
 
+// Which rows and chunks: the time of a launch is estimated (us) from what a
+// workgroup of 32 * waves rows costs, workgroup + step * tiles. The step is the
+// larger of a lone workgroup's and its share of a CU's rate where k workgroups are on
+// the CU (up to per_cu).
+//   one length   the rounds in which the device runs the workgroups;
+//   ragged       the larger of the longest workgroup and the average over the
+//                device's places, plus a share of the smaller (what remains of one
+//                when the other ends). Only the device knows the lengths: their mean
+//                is taken as `filled` of the longest.
+// Not below what reading the keys once takes, plus the join's time. The constants are
+// fits to 950 drawn shapes (1 to 192 sequences, 1 to 32768 keys, 1 to 64 heads, one
+// new token to chunks of 4096), each at every rows and chunks of the lists below. The
+// choice takes 1.026 (head_dim 64) and 1.042 (128) times the best one's time in the
+// geometric mean, more than 1.2 times it at 30 of the 950. Without the 64-row
+// workgroups 1.033 and 1.063; 256 rows are of no use at head_dim 64.
+struct RowsCost
+{
+    int waves, per_cu;
+    float workgroup, step, shared;
+};
+
+struct Costs
+{
+    RowsCost rows[3];
+    int count;
+    float filled, share, join, join_mb, launch, bytes_per_us;  // join_mb: per 10^6 floats of partial results
+};
+
+constexpr Costs kCosts64 = {{{2, 6, 3.66f, 0.352f, 0.158f}, {4, 3, 3.638f, 0.324f, 0.172f}},
+                            2, 0.61f, 0.582f, 4.623f, 1.617f, 3.158f, 4.761e6f};
+constexpr Costs kCosts128 = {{{2, 3, 3.738f, 0.436f, 0.27f}, {4, 2, 3.662f, 0.554f, 0.329f}, {8, 1, 4.357f, 0.552f, 0.228f}},
+                             3, 0.61f, 0.36f, 2.48f, 1.392f, 1.772f, 5.892e6f};
+constexpr int kSplitChoices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
+static_assert(kSplitChoices[15] == kMaxSplits, "the joins' limit");
+
 Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int head_dim, int max_queries, int max_keys,
                bool paged)
 {
-    Plan p{};
-    max_keys = static_cast<int>(std::min<long long>(max_keys, kMaxKeys));
+    const Costs& costs = head_dim == 64 ? kCosts64 : kCosts128;
     const int group = heads / heads_kv;
-    const long long rows = static_cast<long long>(std::min<long long>(max_queries, tokens)) * group;
-    p.waves = rows <= 32 ? 4 : rows <= 64 ? 4 : rows <= 128 ? 4 : 8;
-    const int R = 32 * p.waves;
-    const long long per_seq = (rows + R - 1) / R;
-    p.per_seq = static_cast<int>(per_seq);
-    p.slots = seqs * per_seq;
-    // Ragged batches: at most one slot per full block of rows and one per sequence.
-    const long long packed = tokens * group / R + seqs;
-    if (paged && per_seq > 1 && packed < p.slots)
+    const long long rows = std::min<long long>(max_queries, tokens) * group;
+    const int tiles = static_cast<int>((std::min<long long>(max_keys, kMaxKeys) + kTileKeys - 1) / kTileKeys);
+    const double cus = fa::device_compute_units();
+    const bool ragged = paged && seqs > 1;
+    const double filled = ragged ? costs.filled : 1.0;
+    const double read = static_cast<double>(seqs) * tiles * kTileKeys * heads_kv * head_dim * 4.0 * filled / costs.bytes_per_us;
+    Plan best{};
+    double best_time = 0.0;
+    for (int x = 0; x < costs.count; ++x)
     {
-        p.per_seq = 0;
-        p.slots = packed;
+        const RowsCost& c = costs.rows[x];
+        Plan p{};
+        p.waves = c.waves;
+        const int R = 32 * c.waves;
+        const long long per_seq = (rows + R - 1) / R;
+        p.per_seq = static_cast<int>(std::min<long long>(per_seq, 1 << 30));
+        p.slots = seqs * per_seq;
+        // Ragged batches: at most one slot per full block of rows and one per sequence.
+        const long long packed = tokens * group / R + seqs;
+        if (paged && per_seq > 1 && packed < p.slots)
+        {
+            p.per_seq = 0;
+            p.slots = packed;
+        }
+        const double blocks = static_cast<double>(p.slots) * heads_kv;
+        int last_chunk = 0;
+        for (const int choice : kSplitChoices)
+        {
+            const int chunk = (tiles + choice - 1) / choice;  // tiles
+            if (choice > 1 && (chunk < 2 || chunk == last_chunk)) continue;
+            last_chunk = chunk;
+            const int splits = chunk > 0 ? (tiles + chunk - 1) / chunk : 1;
+            auto step_at = [&](double k) {
+                return std::max<double>(c.step, c.shared * std::min<double>(std::max(k, 1.0), c.per_cu));
+            };
+            const double active = blocks * (splits == 1 ? 1.0 : ragged ? splits * filled : splits);
+            double busy;
+            if (ragged)
+            {
+                const double k = std::min<double>(std::max(active / cus, 1.0), c.per_cu);
+                const double longest = c.workgroup + step_at(k) * chunk;
+                const double average = (active * c.workgroup + blocks * tiles * filled * step_at(k)) / (cus * k);
+                busy = std::max(longest, average) + costs.share * std::min(longest, average);
+            }
+            else
+            {
+                const double rounds = std::floor(active / (cus * c.per_cu));
+                const double rest = active - rounds * cus * c.per_cu;
+                busy = rounds * (c.workgroup + step_at(c.per_cu) * chunk) +
+                       (rest > 0.0 ? c.workgroup + step_at(rest / cus) * chunk : 0.0);
+            }
+            // A smooth maximum: one of the two hides little of the other where they are close.
+            const double busy2 = busy * busy, read2 = read * read;
+            double time = std::sqrt(std::sqrt(busy2 * busy2 + read2 * read2)) + costs.launch;
+            if (splits > 1) time += costs.join + costs.join_mb * 1e-6 * static_cast<double>(tokens) * heads * head_dim * splits;
+            if (best_time == 0.0 || time < best_time)
+            {
+                best_time = time;
+                best = p;
+                best.splits = splits;
+                best.chunk = std::max(chunk, 1) * kTileKeys;
+            }
+        }
     }
-    const long long blocks = p.slots * heads_kv;
-    const long long cus = fa::device_compute_units();
-    const long long target = cus * (p.waves == 2 ? 4 : p.waves == 4 ? 2 : 1);
-    const long long least = 256;  // keys per chunk
-    long long splits = std::max<long long>(1, std::min<long long>({target / std::max<long long>(1, blocks),
-                                                                   (max_keys + least - 1) / least, kMaxSplits}));
-    p.chunk = static_cast<int>(((max_keys + splits - 1) / splits + kTileKeys - 1) / kTileKeys * kTileKeys);
-    p.chunk = std::max(p.chunk, kTileKeys);
-    p.splits = static_cast<int>(std::max<long long>(1, (max_keys + static_cast<long long>(p.chunk) - 1) / p.chunk));
-    if (p.splits > 1) p.workspace = static_cast<size_t>(tokens) * heads * p.splits * (head_dim + 2) * sizeof(float);
-    return p;
+    if (best.splits > 1) best.workspace = static_cast<size_t>(tokens) * heads * best.splits * (head_dim + 2) * sizeof(float);
+    return best;
 }
 
 template <typename T, int D, int kWaves, bool kPaged>
@@ -982,8 +1058,10 @@ int launch_waves(const Args& a, const Plan& p, int head_rows, hipStream_t stream
     {
         case 2: return launch_typed<T, D, 2, kPaged>(a, p, head_rows, stream);
         case 4: return launch_typed<T, D, 4, kPaged>(a, p, head_rows, stream);
-        default: return launch_typed<T, D, 8, kPaged>(a, p, head_rows, stream);
+        default: break;
     }
+    if constexpr (D == 128) return launch_typed<T, D, 8, kPaged>(a, p, head_rows, stream);
+    return hipErrorInvalidValue;  // make_plan names no such rows
 }
 
 template <bool kPaged>
