@@ -276,6 +276,7 @@ struct Rows
     int t_begin, t_end;  // the workgroup's tiles (equal where nothing is seen)
     int t_last;   // the wave's tiles end here
     int t_mask;   // first tile that some lane does not see whole
+    bool unseen;  // some lane does not see keys that the block reads
 };
 
 template <int R>
@@ -294,7 +295,9 @@ __device__ __forceinline__ Rows wave_rows(const Args& a, const Block& b, int spl
     const int first = b.row0 + 32 * wave;
     const int wave_end = first < b.rows ? limit_of(a, b, min(first + 31, b.rows - 1) / a.group) : 0;
     r.t_last = uniform(min(r.t_end, (wave_end + kTileKeys - 1) / kTileKeys));
-    r.t_mask = uniform(limit_of(a, b, min(first, b.rows - 1) / a.group) / kTileKeys);
+    const int least = uniform(limit_of(a, b, min(first, b.rows - 1) / a.group));
+    r.t_mask = least / kTileKeys;
+    r.unseen = least < b.end;
     return r;
 }
 
@@ -665,6 +668,20 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         barrier();
         load_k(1, 0, D / 16);
 
+        // A weight of 0 times an infinity or a NaN is NaN. A tile that some lane does not
+        // see whole (at most two of a wave: its rows' limits lie within 32 keys) is left
+        // out where V holds such values, and added key by key after the walk, to the
+        // lanes that see the key.
+        unsigned left_out = 0;  // bit x: tile t_mask + x
+        auto leave_out = [&](int t) __attribute__((always_inline)) {
+            uint32_t found = 0;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) found |= not_finite<T>(va[x % (D / 32)][x / (D / 32)]);
+            if (!__any(found != 0)) return false;
+            left_out |= 1u << (t - r.t_mask);
+            return true;
+        };
+
         // The base lags (see above): tile jj's P was zeroed; its scores again, the base
         // at the row maximum, O and l rescaled, its P V from V's stage (intact until the
         // next step's copies), and the first half of the next tile's exponentials again.
@@ -750,13 +767,22 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
             fa::wait_vm_lgkm0<(2 * kStages - 5) * kI>();
             barrier();
             // Block B
-            const bool rare = __any(tsum > __builtin_bit_cast(float, limit_bits));
-            if (rare)
+            bool rare = __any(tsum > __builtin_bit_cast(float, limit_bits));
+            bool out = false;
+            if constexpr (kPaged && decltype(masked_tag)::value)  // an encoder's states are seen by all rows
+                if (r.unseen && t0 + jj >= r.t_mask && leave_out(t0 + jj))
+                {
+                    out = true;
+                    rare = false;
+                }
+            if (rare || out)
             {
                 asm volatile("");  // a branch, not selects on the common path
                 p_lo[B] = x8{};
                 p_hi = x8{};
                 tsum = 0.0f;
+#pragma unroll
+                for (int x = 0; x < D / 16; ++x) va[x % (D / 32)][x / (D / 32)] = x8{};  // 0 times an infinity is NaN
             }
             l += tsum;
             // Past the wave's last tile the next scores are of a stage that nobody needs.
@@ -799,6 +825,55 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
             behind = ahead;
             ahead = place_of(t0 + jj + kStages + 1);
             fetch_pages(t0 + jj + kStages + 2);
+        }
+        // The tiles that were left out, a key at a time.
+        for (int t = r.t_mask; kPaged && left_out != 0; ++t, left_out >>= 1)
+        {
+            if ((left_out & 1u) == 0) continue;
+            const int last = min(t * kTileKeys + kTileKeys, b.end);
+            for (int key = t * kTileKeys; key < last; ++key)
+            {
+                const auto at = keys.half_at(key, keys.page_of(key));
+                const bool there = at.k_bytes != 0;  // else a page of zeros
+                float s = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                {
+                    const x8 kx = there ? *reinterpret_cast<const x8*>(at.k + (16 * ks + 8 * h) * 2) : x8{};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s = fmaf(static_cast<float>(kx[e]), static_cast<float>(qr[ks][e]), s);
+                }
+                float sa, sb;
+                row_halves(s, sa, sb);
+                s = sa + sb;
+                const bool sees = key < r.limit;
+                const float m_new = __builtin_elementwise_maximum(m, sees ? s * c_log2 - E::kBias : m);
+                const float alpha = m_new == m ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                float x;
+                {
+#pragma clang fp contract(off)
+                    x = s * c_log2 - m;
+                }
+                const T w = static_cast<T>(sees ? __builtin_amdgcn_exp2f(x) : 0.0f);
+                // Each half of the lanes adds half of a row's keys to its sum: this one,
+                // which both know, is the lower half's.
+                l = l * alpha + (h == 0 ? static_cast<float>(w) : 0.0f);
+#pragma unroll
+                for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                    {
+                        typedef T t4 __attribute__((ext_vector_type(4)));
+                        const t4 vx = there ? *reinterpret_cast<const t4*>(at.v + (32 * db + 8 * g + 4 * h) * 2) : t4{};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                        {
+                            const float grown = o[db][4 * g + e] * alpha;
+                            o[db][4 * g + e] = sees ? fmaf(static_cast<float>(w), static_cast<float>(vx[e]), grown) : grown;
+                        }
+                    }
+            }
         }
         // Every copy has landed and every wave has read its last tile: the stages are free.
         fa::wait_vm_lgkm0<0>();

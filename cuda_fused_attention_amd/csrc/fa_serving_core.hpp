@@ -30,6 +30,7 @@ template <>
 struct Elem<__bf16>
 {
     using x8 = bf16x8;
+    static constexpr uint32_t kExponent = 0x7f80;  // all ones: infinite or NaN
     // bf16 has fp32's range: the largest weight of a row is 1.
     static constexpr float kBias = 0.0f;
     static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c)
@@ -48,6 +49,7 @@ template <>
 struct Elem<_Float16>
 {
     using x8 = f16x8;
+    static constexpr uint32_t kExponent = 0x7c00;
     // fp16 ends at 2^-24 (spacing of its subnormals): with the largest weight
     // at 2^8 instead of 1 a key keeps all 11 bits down to 2^-22 of the
     // largest, and is lost only below 2^-33 of it. 2^8 is far from fp16's
@@ -150,6 +152,20 @@ __device__ __forceinline__ void mask_tile(f32x16& s, int limit)
         const float x = s[r];
         s[r] = (8 * (r >> 2) + (r & 3) < limit) ? x : -INFINITY;
     }
+}
+
+// Whether one of an operand's values is infinite or NaN: bits 15 and 31 of the
+// result (an exponent of ones carries into them; nothing else does).
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(typename Elem<T>::x8 v)
+{
+    constexpr uint32_t kMask = Elem<T>::kExponent * 0x10001u;
+    constexpr uint32_t kOne = (0x8000u - Elem<T>::kExponent) * 0x10001u;
+    const i32x4 bits = __builtin_bit_cast(i32x4, v);
+    uint32_t found = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) found |= (static_cast<uint32_t>(bits[e]) & kMask) + kOne;
+    return found & 0x80008000u;
 }
 
 // The exponent base of a row that has seen no key: every finite scaled score is

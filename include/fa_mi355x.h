@@ -350,8 +350,9 @@ int fa_launch_paged_append(const void* k, const void* v, const long long* slot_m
  * row that sees no key is 0. Rows of no sequence, and those past the first
  * max_query_len of one, are left as they were. Keys past table_width *
  * block_size do not exist; a table entry outside the cache stands for a page of
- * zeros. What a page holds behind its sequence's length is never used. head_dim
- * 64 or 128 (else FA_ERROR_UNSUPPORTED).
+ * zeros. What a page holds behind its sequence's length is never used, and a key or
+ * value that is not finite reaches the rows that see it and no other (an infinity in
+ * V whose weight rounds to 0 gives NaN). head_dim 64 or 128 (else FA_ERROR_UNSUPPORTED).
  * max_query_len: no sequence has more new tokens. max_kv_len: about the most keys
  * of one; it only decides how the work is split, any value gives the same
  * result up to rounding. workspace: fa_attention_paged_workspace_bytes of the

@@ -333,6 +333,85 @@ def test_paged_large_scores(fa, dtype):
     b.check(fa, True, "large scores")
 
 
+def _check_not_finite(b, got, causal):
+    """Rows against sums over the keys that each sees: infinities and NaN where one of
+    those holds them, the usual tolerance elsewhere. fp16 weights are multiples of 2^-24
+    where the row's largest is 2^8 or more, so a key of less than 2^-33 of the largest
+    weighs 0, and 0 times an infinity is NaN: below 2^-32 either is right."""
+    heads, group = b.q.shape[1], b.q.shape[1] // b.k.shape[1]
+    clean_v = torch.where(b.v.isfinite(), b.v, 0)
+    clean_k = torch.where(b.k.isfinite(), b.k, 0)
+    want, tol, _ = ref.paged(b.q, clean_k, clean_v, b.table, b.starts, b.kv, b.block, causal)
+    for s, kv in enumerate(b.kv):
+        a, n = b.starts[s], b.starts[s + 1] - b.starts[s]
+        pos = torch.arange(kv, device="cuda")
+        page = b.table[s].long()[pos // b.block]
+        first = kv - n + 1 if causal else kv
+        for h in range(heads):
+            v = b.v[page, h // group, pos % b.block].double()
+            bad_k = ~b.k[page, h // group, pos % b.block].isfinite().all(-1)
+            for i in range(n):
+                seen = slice(0, first + (i if causal else 0))
+                extra = torch.where(v[seen].isfinite(), 0.0, v[seen]).sum(0)
+                if bad_k[seen].any():
+                    extra = torch.full_like(extra, float("nan"))
+                got_row, want_row, t = got[a + i, h].double(), want[a + i, h], tol[a + i, h]
+                fine = extra == 0
+                inf = extra.isinf()
+                if b.dtype == torch.float16 and inf.any():
+                    k = clean_k[page, h // group, pos % b.block].double()[seen]
+                    score = torch.mv(k, b.q[a + i, h].double()) / math.sqrt(k.shape[1])
+                    lost = score - score.amax() < -32 * math.log(2)
+                    vanished = (v[seen].isinf() & lost[:, None]).any(0)
+                    assert (got_row[inf & vanished].isinf() | got_row[inf & vanished].isnan()).all(), (s, i, h)
+                    got_row = torch.where(vanished, extra, got_row)
+                assert (got_row.isnan() == extra.isnan()).all(), (s, i, h)
+                assert (got_row[inf] == extra[inf]).all(), (s, i, h)
+                ref.check(got_row[fine], want_row[fine], t[fine], f"sequence {s} row {i} head {h}")
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("fp16", 128), ("bf16", 128)])
+@pytest.mark.parametrize("scale", [1.0, 3.0])
+def test_paged_infinities_and_nan_in_v(fa, dtype, dim, scale):
+    """A value that is not finite reaches the rows that see its key, and no other: in
+    the tile of the diagonal, beside it, with rising scores, and a page of zeros there."""
+    for cached, new, heads, heads_kv in (([0, 13], [40, 33], 2, 1), ([100], [70], 2, 2), ([5, 0], [3, 140], 4, 1)):
+        b = Paged(fa, cached, new, heads, heads_kv, dim, 16, dtype, seed=21, scale=scale, extra_rows=1)
+        for s, (at, value, d) in enumerate([(-1, math.nan, 3), (-2, math.inf, 7), (-20, -math.inf, 11), (-33, math.inf, 11)]):
+            for q in range(len(new)):
+                p = b.kv[q] + at
+                if p >= 0:
+                    b.v[b.table[q, p // 16], :, p % 16, d + 16 * (s % 2)] = value
+        say("not finite v", dtype, dim, scale, cached, new)
+        _check_not_finite(b, b.run(fa), True)
+        _check_not_finite(b, b.run(fa, max_kv_len=4096), True)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_paged_not_finite_keys(fa, value):
+    """A key that is not finite makes the rows that see it NaN, and no other."""
+    b = Paged(fa, [20, 3], [70, 35], 2, 1, 64, 16, "bf16", seed=5)
+    for q, p in ((0, 60), (1, 37)):
+        b.k[b.table[q, p // 16], :, p % 16, 5] = math.nan
+    b.v[b.table[0, 50 // 16], :, 50 % 16, 9] = value
+    say("not finite k", value)
+    _check_not_finite(b, b.run(fa), True)
+
+
+def test_paged_left_out_tile_with_a_missing_page(fa):
+    """The tile of the diagonal holds a NaN, and half of it lies in a page of zeros."""
+    b = Paged(fa, [0], [64], 2, 1, 64, 16, "bf16", seed=6)
+    b.v[b.table[0, 3], :, 15, 4] = math.nan
+    b.table[0, 2] = -1
+    say("left out, missing page")
+    got = b.run(fa)
+    v = b.v.clone()
+    v[b.table[0, 3], :, 15, 4] = 0
+    want, tol, _ = ref.paged(b.q, b.k, v, b.table, b.starts, b.kv, 16, True)
+    assert got[63, :, 4].isnan().all()
+    ref.check(got[:63], want[:63], tol[:63], "left out")
+
+
 # ---------------------------------------------------------------- attention to an encoder's states
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("dim", [64, 128])
