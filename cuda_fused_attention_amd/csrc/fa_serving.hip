@@ -502,9 +502,13 @@ constexpr float kSumLimit<_Float16> = 32768.0f;
 // (fp32's spacing at 2^28 is 32): every tile takes the exact path.
 constexpr float kCoarseBase = 268435456.0f;
 
-template <typename T, int D, int kWaves, bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWaves > 2 ? 2 : 1, 8))) void serving_attention_kernel(
-    const Args a)
+// Workgroups of a CU that the stages leave room for.
+template <int D, int kGroups>
+constexpr int kGroupsPerCu = 160 * 1024 / (kGroups * 6 * kTileKeys * D * 2);
+
+template <typename T, int D, int kWaves, int kGroups, bool kPaged>
+__global__ __launch_bounds__(64 * kWaves * kGroups)
+__attribute__((amdgpu_waves_per_eu(kWaves * kGroups > 2 && kGroupsPerCu<D, kGroups> > 1 ? 2 : 1, 8))) void serving_attention_kernel(const Args a)
 {
     using E = Elem<T>;
     using x8 = typename E::x8;
@@ -516,24 +520,37 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
     constexpr int kI = C::kIssues;
     // A wave's copies of a tile lie in one half of it, or in both.
     constexpr int kHalves = kI > 1 ? 2 : 1;
-    constexpr int kStoreElems = kWaves * 2048;  // 4 KiB a wave at the end (store_rows)
-    constexpr int kLdsElems = 2 * kStages * kTile > kStoreElems ? 2 * kStages * kTile : kStoreElems;
+    constexpr int kGroupElems = 2 * kStages * kTile;
+    // At the end the stages' room holds the second group's results (two groups) and
+    // 4 KiB a wave for the stores.
+    constexpr int kOtFloats = (D / 32) * 16 * 64;  // one wave's O^T
+    constexpr int kMergeElems = kGroups == 1 ? 0 : kWaves * (kOtFloats + 128) * 2;
+    constexpr int kEndElems = kMergeElems + kWaves * 2048;
+    constexpr int kLdsElems = kGroups * kGroupElems > kEndElems ? kGroups * kGroupElems : kEndElems;
     __shared__ __attribute__((aligned(16))) uint16_t lds[kLdsElems];
 
     const int lane = threadIdx.x & 63;
-    const int wave = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int wave_all = uniform(static_cast<int>(threadIdx.x >> 6));
+    const int grp = kGroups == 1 ? 0 : wave_all / kWaves;
+    const int wave = kGroups == 1 ? wave_all : wave_all % kWaves;
     const int i = lane & 31;
     const int h = lane >> 5;
     Block b;
     int split;
     if (!take_block<R, kPaged>(a, b, split)) return;
-    const Rows r = wave_rows<R>(a, b, split, wave, i);
+    Rows r = wave_rows<R>(a, b, split, wave, i);
+    const bool any_tile = r.t_begin < r.t_end;
+    // Two groups: each walks half of the tiles, with the same number of steps.
+    const int steps = (r.t_end - r.t_begin + kGroups - 1) / kGroups;
+    r.t_begin += grp * steps;
+    r.t_end = min(r.t_end, r.t_begin + steps);
+    r.t_last = min(r.t_last, r.t_end);
 
     f32x16 o[D / 32];
 #pragma unroll
     for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
     float m = kEmptyBase, l = 0.0f;
-    if (r.t_begin < r.t_end)
+    if (any_tile)
     {
         const Keys<D, kPaged> keys(a, b);
         const float c_log2 = a.c_log2;
@@ -550,7 +567,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
                 voff[u] = static_cast<uint32_t>(row & 15) * keys.v_row_bytes + ((pchunk ^ swz_v<D>(row)) * 16);
             }
         }
-        const uint32_t lds_base = fa::lds_addr(lds);
+        const uint32_t lds_base = fa::lds_addr(lds) + grp * (kGroupElems * 2);
         const int half0 = kHalves == 1 ? (wave * C::kRows) & 16 : 0;  // first key of the wave's (first) half
         struct Place
         {
@@ -584,7 +601,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         static_assert(kHalves == 1 || 16 % (kWaves * C::kRows) == 0, "every wave's copy u lies in the same half");
 
         const int t0 = r.t_begin;
-        const int cnt = r.t_end - t0;
+        const int cnt = steps;
         const int lw = r.t_last - t0 - 1;             // last step this wave computes
         const int j_mask = min(lw, r.t_mask - t0 - 1);  // first step whose next tile is masked
 
@@ -618,9 +635,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
 
         int k_at[D / 16], v_at[D / 32];  // byte offsets, pinned at each use: the stage then folds into the read
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) k_at[ks] = 2 * k_read_offset<D>(i, h, ks);
+        for (int ks = 0; ks < D / 16; ++ks) k_at[ks] = 2 * (grp * kGroupElems + k_read_offset<D>(i, h, ks));
 #pragma unroll
-        for (int db = 0; db < D / 32; ++db) v_at[db] = 2 * (kStages * kTile + v_read_offset<D>(lane, db));
+        for (int db = 0; db < D / 32; ++db) v_at[db] = 2 * (grp * kGroupElems + kStages * kTile + v_read_offset<D>(lane, db));
         x8 ka[D / 16], va[D / 32][2];
         auto load_k = [&](int stage, int first, int count) {
 #pragma unroll
@@ -879,8 +896,40 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kWa
         fa::wait_vm_lgkm0<0>();
         barrier();
     }
+    if constexpr (kGroups == 2)
+    {
+        // The second group hands its O^T, base and sum to the first.
+        float* const part = reinterpret_cast<float*>(lds) + wave * (kOtFloats + 128);
+        if (grp == 1)
+        {
+#pragma unroll
+            for (int x = 0; x < D / 8; ++x)
+            {
+                const f32x16& ob = o[x / 4];
+                *reinterpret_cast<f32x4*>(part + (x * 64 + lane) * 4) =
+                    f32x4{ob[4 * (x % 4)], ob[4 * (x % 4) + 1], ob[4 * (x % 4) + 2], ob[4 * (x % 4) + 3]};
+            }
+            part[kOtFloats + lane] = m;
+            part[kOtFloats + 64 + lane] = l;
+        }
+        fa::wait_vm_lgkm0<63>();
+        barrier();
+        if (grp == 1) return;
+        const float m1 = part[kOtFloats + lane], l1 = part[kOtFloats + 64 + lane];
+        const float top = __builtin_elementwise_maximum(m, m1);
+        const float w0 = __builtin_amdgcn_exp2f(m - top), w1 = __builtin_amdgcn_exp2f(m1 - top);
+        l = l * w0 + l1 * w1;
+        m = top;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x)
+        {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(part + (x * 64 + lane) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[x / 4][4 * (x % 4) + e] = o[x / 4][4 * (x % 4) + e] * w0 + y[e] * w1;
+        }
+    }
     if (b.row0 + 32 * wave < b.rows)
-        store_rows<T, D, kPaged>(a, b, r, split, lane, o, m, l, reinterpret_cast<uint4*>(lds) + wave * 256);
+        store_rows<T, D, kPaged>(a, b, r, split, lane, o, m, l, reinterpret_cast<uint4*>(lds + kMergeElems) + wave * 256);
 }
 
 // Joins the chunks of a row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c with
@@ -993,7 +1042,7 @@ __global__ __launch_bounds__(256) void serving_join_kernel(const Args a, int blo
 // Rows of a workgroup, row blocks and key chunks of a launch.
 struct Plan
 {
-    int waves;
+    int waves, groups;
     int per_seq;
     long long slots;
     int splits, chunk;
@@ -1010,28 +1059,33 @@ struct Plan
 //                when the other ends). Only the device knows the lengths: their mean
 //                is taken as `filled` of the longest.
 // Not below what reading the keys once takes, plus the join's time. The constants are
-// fits to 950 drawn shapes (1 to 192 sequences, 1 to 32768 keys, 1 to 64 heads, one
+// fits to 1020 drawn shapes (1 to 192 sequences, 1 to 32768 keys, 1 to 64 heads, one
 // new token to chunks of 4096), each at every rows and chunks of the lists below. The
-// choice takes 1.026 (head_dim 64) and 1.042 (128) times the best one's time in the
-// geometric mean, more than 1.2 times it at 30 of the 950. Without the 64-row
-// workgroups 1.033 and 1.063; 256 rows are of no use at head_dim 64.
+// choice takes 1.031 (head_dim 64) and 1.046 (128) times the best one's time in the
+// geometric mean, more than 1.2 times it at 39 of the 1020. Without the two groups it
+// would be 1.038 and 1.064; two groups of 128 rows gain 0.4 % and are not built, and
+// 256 rows are of no use at head_dim 64.
 struct RowsCost
 {
-    int waves, per_cu;
+    int waves, groups, per_cu;
     float workgroup, step, shared;
 };
 
 struct Costs
 {
-    RowsCost rows[3];
+    RowsCost rows[4];
     int count;
     float filled, share, join, join_mb, launch, bytes_per_us;  // join_mb: per 10^6 floats of partial results
 };
 
-constexpr Costs kCosts64 = {{{2, 6, 3.66f, 0.352f, 0.158f}, {4, 3, 3.638f, 0.324f, 0.172f}},
-                            2, 0.61f, 0.582f, 4.623f, 1.617f, 3.158f, 4.761e6f};
-constexpr Costs kCosts128 = {{{2, 3, 3.738f, 0.436f, 0.27f}, {4, 2, 3.662f, 0.554f, 0.329f}, {8, 1, 4.357f, 0.552f, 0.228f}},
-                             3, 0.61f, 0.36f, 2.48f, 1.392f, 1.772f, 5.892e6f};
+constexpr Costs kCosts64 = {
+    {{2, 1, 6, 2.857f, 0.454f, 0.131f}, {4, 1, 3, 2.849f, 0.365f, 0.151f}, {2, 2, 3, 3.68f, 0.384f, 0.205f}},
+    3, 0.9f, 0.507f, 4.118f, 1.335f, 1.95f, 5.958e6f};
+constexpr Costs kCosts128 = {{{2, 1, 3, 3.076f, 0.527f, 0.301f},
+                              {4, 1, 2, 2.753f, 0.749f, 0.285f},
+                              {8, 1, 1, 3.781f, 0.676f, 0.4f},
+                              {2, 2, 1, 3.998f, 0.648f, 0.394f}},
+                             4, 0.9f, 0.601f, 2.864f, 1.855f, 3.612f, 6.901e6f};
 constexpr int kSplitChoices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 static_assert(kSplitChoices[15] == kMaxSplits, "the joins' limit");
 
@@ -1053,6 +1107,7 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
         const RowsCost& c = costs.rows[x];
         Plan p{};
         p.waves = c.waves;
+        p.groups = c.groups;
         const int R = 32 * c.waves;
         const long long per_seq = (rows + R - 1) / R;
         p.per_seq = static_cast<int>(std::min<long long>(per_seq, 1 << 30));
@@ -1076,20 +1131,21 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
                 return std::max<double>(c.step, c.shared * std::min<double>(std::max(k, 1.0), c.per_cu));
             };
             const double active = blocks * (splits == 1 ? 1.0 : ragged ? splits * filled : splits);
+            const int steps = (chunk + c.groups - 1) / c.groups;
             double busy;
             if (ragged)
             {
                 const double k = std::min<double>(std::max(active / cus, 1.0), c.per_cu);
-                const double longest = c.workgroup + step_at(k) * chunk;
-                const double average = (active * c.workgroup + blocks * tiles * filled * step_at(k)) / (cus * k);
+                const double longest = c.workgroup + step_at(k) * steps;
+                const double average = (active * c.workgroup + blocks * tiles / c.groups * filled * step_at(k)) / (cus * k);
                 busy = std::max(longest, average) + costs.share * std::min(longest, average);
             }
             else
             {
                 const double rounds = std::floor(active / (cus * c.per_cu));
                 const double rest = active - rounds * cus * c.per_cu;
-                busy = rounds * (c.workgroup + step_at(c.per_cu) * chunk) +
-                       (rest > 0.0 ? c.workgroup + step_at(rest / cus) * chunk : 0.0);
+                busy = rounds * (c.workgroup + step_at(c.per_cu) * steps) +
+                       (rest > 0.0 ? c.workgroup + step_at(rest / cus) * steps : 0.0);
             }
             // A smooth maximum: one of the two hides little of the other where they are close.
             const double busy2 = busy * busy, read2 = read * read;
@@ -1108,18 +1164,18 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
     return best;
 }
 
-template <typename T, int D, int kWaves, bool kPaged>
+template <typename T, int D, int kWaves, int kGroups, bool kPaged>
 int launch_typed(const Args& a, const Plan& p, int head_rows, hipStream_t stream)
 {
     const long long blocks = p.slots * a.heads_kv * p.splits;
-    if (blocks > 0x7fffffffLL / (64 * kWaves)) return hipErrorInvalidValue;
+    if (blocks > 0x7fffffffLL / (64 * kWaves * kGroups)) return hipErrorInvalidValue;
     const int block_rows = std::min(32 * kWaves, head_rows);
     const bool alone = block_rows <= kAloneRows;
     const int parts = alone ? block_rows : (block_rows + kJoinRows - 1) / kJoinRows;
     const long long join_blocks = p.slots * a.heads_kv * parts;
     if (p.splits > 1 && join_blocks > 0x7fffffffLL / 256) return hipErrorInvalidValue;
-    const hipError_t e = fa::launch_kernel(serving_attention_kernel<T, D, kWaves, kPaged>,
-                                           dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), stream, a);
+    const hipError_t e = fa::launch_kernel(serving_attention_kernel<T, D, kWaves, kGroups, kPaged>,
+                                           dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves * kGroups), stream, a);
     if (e != hipSuccess || p.splits == 1) return e;
     return fa::launch_kernel(alone ? serving_join_kernel<T, D, 32 * kWaves, kPaged, true>
                                    : serving_join_kernel<T, D, 32 * kWaves, kPaged, false>,
@@ -1129,14 +1185,12 @@ int launch_typed(const Args& a, const Plan& p, int head_rows, hipStream_t stream
 template <typename T, int D, bool kPaged>
 int launch_waves(const Args& a, const Plan& p, int head_rows, hipStream_t stream)
 {
-    switch (p.waves)
-    {
-        case 2: return launch_typed<T, D, 2, kPaged>(a, p, head_rows, stream);
-        case 4: return launch_typed<T, D, 4, kPaged>(a, p, head_rows, stream);
-        default: break;
-    }
-    if constexpr (D == 128) return launch_typed<T, D, 8, kPaged>(a, p, head_rows, stream);
-    return hipErrorInvalidValue;  // make_plan names no such rows
+    if (p.waves == 2 && p.groups == 1) return launch_typed<T, D, 2, 1, kPaged>(a, p, head_rows, stream);
+    if (p.waves == 4 && p.groups == 1) return launch_typed<T, D, 4, 1, kPaged>(a, p, head_rows, stream);
+    if (p.waves == 2 && p.groups == 2) return launch_typed<T, D, 2, 2, kPaged>(a, p, head_rows, stream);
+    if constexpr (D == 128)
+        if (p.waves == 8 && p.groups == 1) return launch_typed<T, D, 8, 1, kPaged>(a, p, head_rows, stream);
+    return hipErrorInvalidValue;  // make_plan names no others
 }
 
 template <bool kPaged>

@@ -135,20 +135,28 @@ def launch_attention_cross(q, k, v, o, workspace, workspace_bytes: int, kv_lens,
 
 
 # ---------------------------------------------------------------- torch convenience
-# torch, the element types and the current device, bound on first use (torch is
-# imported only for torch callers). These functions are on the path of every
-# decoding step, so a check costs its comparisons and builds no message.
+# torch, the element types, the current device and its current stream as raw values,
+# and the library, bound on first use (torch is imported only for torch callers).
+# These functions are on the path of every decoding step: they call the C entry
+# points without the wrappers above, and a check costs its comparisons and builds no
+# message (7.8 -> 6 us for paged_slots, of which its kernel's launch is 3.5).
 _torch = None
 _dtype_ids = {}
-_current_device = None
+_device_index = None
+_raw_stream = None
+_lib = None
 
 
 def _bind():
-    global _torch, _dtype_ids, _current_device
+    global _torch, _dtype_ids, _device_index, _raw_stream, _lib
     import torch
 
     _dtype_ids = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_FP16}
-    _current_device = torch.cuda.current_device
+    _device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if _raw_stream is None:
+        _raw_stream = lambda index: int(torch.cuda.current_stream(index).cuda_stream)  # noqa: E731
+    _lib = _fa.lib()
     _torch = torch
     return torch
 
@@ -159,11 +167,11 @@ def _dtype_id(dtype) -> int:
     return _dtype_ids[dtype]
 
 
-def _elsewhere(device) -> bool:
-    """Whether `device` is another GPU than the current one."""
+def _other_device(device):
+    """A context in which `device`, another GPU than the current one, is current."""
     if device.type != "cuda":
         raise ValueError("CUDA tensors are needed")
-    return device.index != _current_device()
+    return _torch.cuda.device(device)
 
 
 def _need(ok: bool, what: str):
@@ -216,10 +224,12 @@ def _workspace_room(workspace, device) -> int:
     return workspace.nbytes
 
 
-def _too_small(workspace, have: int, nbytes: int):
-    """Says so where a refused launch's workspace was too small."""
-    if workspace is not None and have < nbytes:
-        raise ValueError(f"workspace holds {have} bytes, {nbytes} are needed")
+def _refused(status: int, what: str, head_dim: int, workspace, have: int, need: int):
+    if status == _fa.FA_ERROR_UNSUPPORTED:
+        raise ValueError(f"head_dim {head_dim} is not supported")
+    if workspace is not None and have < need:
+        raise ValueError(f"workspace holds {have} bytes, {need} are needed")
+    raise _fa.FaError(status, what)
 
 
 def paged_cache(k_cache, v_cache) -> PagedCache:
@@ -259,8 +269,9 @@ def paged_slots(cached_lens, new_lens, block_table, free_blocks, block_size: int
     All int32; what happens at the ends is written at fa_launch_paged_slots."""
     torch = _torch or _bind()
     device = cached_lens.device
-    if _elsewhere(device):
-        with torch.cuda.device(device):
+    index = device.index
+    if index is None or index != _device_index():
+        with _other_device(device):
             return paged_slots(cached_lens, new_lens, block_table, free_blocks, block_size, max_tokens, out)
     num_seqs, num_free = cached_lens.numel(), free_blocks.numel()
     if out is None:
@@ -272,8 +283,12 @@ def paged_slots(cached_lens, new_lens, block_table, free_blocks, block_size: int
     _vector(new_lens, num_seqs, device, int32, "new_lens")
     _vector(free_blocks, num_free, device, int32, "free_blocks")
     width, stride = _table(block_table, num_seqs, device)
-    launch_paged_slots(cached_lens, new_lens, block_table, free_blocks, out.query_starts, out.kv_lens, out.slot_map,
-                       out.blocks_taken, num_seqs, width, stride, num_free, block_size, max_tokens)
+    status = _lib.fa_launch_paged_slots(
+        cached_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_blocks.data_ptr(),
+        out.query_starts.data_ptr(), out.kv_lens.data_ptr(), out.slot_map.data_ptr(), out.blocks_taken.data_ptr(), num_seqs,
+        width, stride, num_free, block_size, max_tokens, _raw_stream(index))
+    if status:
+        raise _fa.FaError(status, "fa_launch_paged_slots")
     return out
 
 
@@ -281,8 +296,9 @@ def paged_append(k, v, slot_map, cache: PagedCache) -> None:
     """New rows k, v [tokens, heads_kv, head_dim] into the cache's slots slot_map
     (int64 [tokens]; negative or past the cache: skipped)."""
     device = cache.device
-    if _elsewhere(device):
-        with _torch.cuda.device(device):
+    index = device.index
+    if index is None or index != _device_index():
+        with _other_device(device):
             return paged_append(k, v, slot_map, cache)
     tokens = slot_map.numel()
     _vector(slot_map, tokens, device, _torch.int64, "slot_map")
@@ -291,7 +307,10 @@ def paged_append(k, v, slot_map, cache: PagedCache) -> None:
     if (k.dtype is not dtype or v.dtype is not dtype or k.shape != shape or v.shape != shape or k.device != device
             or v.device != device):
         raise ValueError(f"k and v must be {dtype} tensors {list(shape)} on {device}")
-    launch_paged_append(k, v, slot_map, cache, tokens, _strides_of(k, "k"), _strides_of(v, "v"))
+    status = _lib.fa_launch_paged_append(k.data_ptr(), v.data_ptr(), slot_map.data_ptr(), cache.ref, tokens,
+                                         _strides(_strides_of(k, "k")), _strides(_strides_of(v, "v")), _raw_stream(index))
+    if status:
+        raise _fa.FaError(status, "fa_launch_paged_append")
 
 
 def attention_paged_workspace(q, cache: PagedCache, num_seqs: int, max_query_len: int, max_kv_len: int):
@@ -314,8 +333,9 @@ def attention_paged(q, cache: PagedCache, block_table, query_starts, kv_lens, ma
     attention_paged_workspace, one per call that may run at the same time; a new one
     if not given. Returns O, like q."""
     device = cache.device
-    if _elsewhere(device):
-        with _torch.cuda.device(device):
+    index = device.index
+    if index is None or index != _device_index():
+        with _other_device(device):
             return attention_paged(q, cache, block_table, query_starts, kv_lens, max_query_len, max_kv_len, causal, out,
                                    workspace)
     if q.dim() != 3 or q.dtype is not cache.dtype or q.device != device:
@@ -334,25 +354,20 @@ def attention_paged(q, cache: PagedCache, block_table, query_starts, kv_lens, ma
     else:
         _like_q(out, q)
 
-    def need():
-        return attention_paged_workspace_bytes(tokens, num_seqs, heads, cache.heads_kv, head_dim, max_query_len, max_kv_len)
-
-    given = workspace
-    if workspace is None:
-        have = need()
-        if have:
-            workspace = _torch.empty(have, dtype=_torch.uint8, device=device)
-    else:
+    room, have = workspace, 0
+    if workspace is not None:
         have = _workspace_room(workspace, device)
-    try:
-        ok = launch_attention_paged(q, cache, out, workspace, have, block_table, query_starts, kv_lens, num_seqs, tokens,
-                                    heads, width, stride, max_query_len, max_kv_len, causal, _strides_of(q, "q"),
-                                    _strides_of(out, "out"))
-    except _fa.FaError:
-        _too_small(given, have, need())
-        raise
-    if not ok:
-        raise ValueError(f"head_dim {head_dim} is not supported")
+    else:
+        have = attention_paged_workspace_bytes(tokens, num_seqs, heads, cache.heads_kv, head_dim, max_query_len, max_kv_len)
+        if have:
+            room = _torch.empty(have, dtype=_torch.uint8, device=device)
+    status = _lib.fa_launch_attention_paged(
+        q.data_ptr(), cache.ref, out.data_ptr(), None if room is None else room.data_ptr(), have, block_table.data_ptr(),
+        query_starts.data_ptr(), kv_lens.data_ptr(), num_seqs, tokens, heads, width, stride, max_query_len, max_kv_len,
+        1 if causal else 0, _strides(_strides_of(q, "q")), _strides(_strides_of(out, "out")), _raw_stream(index))
+    if status:
+        need = attention_paged_workspace_bytes(tokens, num_seqs, heads, cache.heads_kv, head_dim, max_query_len, max_kv_len)
+        _refused(status, "fa_launch_attention_paged", head_dim, workspace, have, need)
     return out
 
 
@@ -373,8 +388,9 @@ def attention_cross(q, k, v, kv_lens=None, out=None, workspace=None):
     one if not given. Returns O, like q."""
     torch = _torch or _bind()
     device = q.device
-    if _elsewhere(device):
-        with torch.cuda.device(device):
+    index = device.index
+    if index is None or index != _device_index():
+        with _other_device(device):
             return attention_cross(q, k, v, kv_lens, out, workspace)
     dtype = q.dtype
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
@@ -392,23 +408,19 @@ def attention_cross(q, k, v, kv_lens=None, out=None, workspace=None):
     else:
         _like_q(out, q)
 
-    def need():
-        return attention_cross_workspace_bytes(batch, heads, heads_kv, q_len, kv_len, head_dim)
-
-    given = workspace
-    if workspace is None:
-        have = need()
-        if have:
-            workspace = torch.empty(have, dtype=torch.uint8, device=device)
-    else:
+    room, have = workspace, 0
+    if workspace is not None:
         have = _workspace_room(workspace, device)
-    try:
-        ok = launch_attention_cross(q, k, v, out, workspace, have, kv_lens, batch, heads, heads_kv, q_len, kv_len, head_dim,
-                                    _dtype_id(dtype), _strides_of(q, "q"), _strides_of(k, "k"), _strides_of(v, "v"),
-                                    _strides_of(out, "out"))
-    except _fa.FaError:
-        _too_small(given, have, need())
-        raise
-    if not ok:
-        raise ValueError(f"head_dim {head_dim} is not supported")
+    else:
+        have = attention_cross_workspace_bytes(batch, heads, heads_kv, q_len, kv_len, head_dim)
+        if have:
+            room = torch.empty(have, dtype=torch.uint8, device=device)
+    status = _lib.fa_launch_attention_cross(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if room is None else room.data_ptr(), have,
+        None if kv_lens is None else kv_lens.data_ptr(), batch, heads, heads_kv, q_len, kv_len, head_dim, _dtype_id(dtype),
+        _strides(_strides_of(q, "q")), _strides(_strides_of(k, "k")), _strides(_strides_of(v, "v")),
+        _strides(_strides_of(out, "out")), _raw_stream(index))
+    if status:
+        need = attention_cross_workspace_bytes(batch, heads, heads_kv, q_len, kv_len, head_dim)
+        _refused(status, "fa_launch_attention_cross", head_dim, workspace, have, need)
     return out
