@@ -135,11 +135,11 @@ _SIGNATURES = {
     "fa_launch_paged_slots": (_i, [_vp] * 8 + [_i, _i, _ll, _i, _i, _i, _vp]),
     "fa_launch_paged_append": (_i, [_vp, _vp, _vp, _cache, _i, _strides, _strides, _vp]),
     "fa_attention_paged_workspace_bytes": (_sz, [_i] * 7),
-    "fa_attention_paged_config": (_i, [_i] * 7 + [_ip, _ip]),
+    "fa_attention_paged_config": (_i, [_i] * 7 + [_ip] * 3),
     "fa_launch_attention_paged": (_i, [_vp, _cache, _vp, _vp, _sz, _vp, _vp, _vp, _i, _i, _i, _i, _ll, _i, _i, _i,
                                        _strides, _strides, _vp]),
     "fa_attention_cross_workspace_bytes": (_sz, [_i] * 6),
-    "fa_attention_cross_config": (_i, [_i] * 6 + [_ip, _ip]),
+    "fa_attention_cross_config": (_i, [_i] * 6 + [_ip] * 3),
     "fa_launch_attention_cross": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _vp] + [_i] * 7 + [_strides] * 4 + [_vp]),
     "fa_build_info": (ctypes.c_char_p, []),
 }

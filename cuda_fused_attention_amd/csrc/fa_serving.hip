@@ -1338,16 +1338,17 @@ size_t fa_attention_paged_workspace_bytes(int tokens, int num_seqs, int heads, i
 }
 
 int fa_attention_paged_config(int tokens, int num_seqs, int heads, int heads_kv, int head_dim, int max_query_len,
-                              int max_kv_len, int* rows_per_block, int* splits)
+                              int max_kv_len, int* rows_per_block, int* kv_groups, int* splits)
 {
-    if (!rows_per_block || !splits) return fa::record_status(hipErrorInvalidValue);
-    *rows_per_block = *splits = 0;
+    if (!rows_per_block || !kv_groups || !splits) return fa::record_status(hipErrorInvalidValue);
+    *rows_per_block = *kv_groups = *splits = 0;
     if (head_dim != 64 && head_dim != 128) return FA_ERROR_UNSUPPORTED;
     if (tokens <= 0 || num_seqs <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || max_query_len <= 0 ||
         max_kv_len < 0)
         return fa::record_status(hipErrorInvalidValue);
     const Plan p = make_plan(num_seqs, tokens, heads, heads_kv, head_dim, max_query_len, max_kv_len, true);
     *rows_per_block = 32 * p.waves;
+    *kv_groups = p.groups;
     *splits = p.splits;
     return hipSuccess;
 }
@@ -1371,15 +1372,16 @@ size_t fa_attention_cross_workspace_bytes(int batch, int heads, int heads_kv, in
 }
 
 int fa_attention_cross_config(int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim,
-                              int* rows_per_block, int* splits)
+                              int* rows_per_block, int* kv_groups, int* splits)
 {
-    if (!rows_per_block || !splits) return fa::record_status(hipErrorInvalidValue);
-    *rows_per_block = *splits = 0;
+    if (!rows_per_block || !kv_groups || !splits) return fa::record_status(hipErrorInvalidValue);
+    *rows_per_block = *kv_groups = *splits = 0;
     if (head_dim != 64 && head_dim != 128) return FA_ERROR_UNSUPPORTED;
     if (batch <= 0 || heads <= 0 || heads_kv <= 0 || heads % heads_kv != 0 || q_len <= 0 || kv_len < 0)
         return fa::record_status(hipErrorInvalidValue);
     const Plan p = make_plan(batch, static_cast<long long>(batch) * q_len, heads, heads_kv, head_dim, q_len, kv_len, false);
     *rows_per_block = 32 * p.waves;
+    *kv_groups = p.groups;
     *splits = p.splits;
     return hipSuccess;
 }

@@ -89,16 +89,16 @@ def attention_paged_workspace_bytes(tokens: int, num_seqs: int, heads: int, head
 
 
 def _config(call, *sizes):
-    rows, splits = ctypes.c_int(), ctypes.c_int()
-    if not _fa._check(getattr(_fa.lib(), call)(*sizes, ctypes.byref(rows), ctypes.byref(splits)), call):
+    out = [ctypes.c_int() for _ in range(3)]
+    if not _fa._check(getattr(_fa.lib(), call)(*sizes, *map(ctypes.byref, out)), call):
         return None
-    return rows.value, splits.value
+    return tuple(x.value for x in out)
 
 
 def attention_paged_config(tokens: int, num_seqs: int, heads: int, heads_kv: int, head_dim: int, max_query_len: int,
                            max_kv_len: int):
-    """(rows per workgroup, most chunks of a sequence's keys), or None for an
-    unsupported head_dim."""
+    """(rows per workgroup, wave groups that share its keys, most chunks of a
+    sequence's keys), or None for an unsupported head_dim."""
     return _config("fa_attention_paged_config", tokens, num_seqs, heads, heads_kv, head_dim, max_query_len, max_kv_len)
 
 

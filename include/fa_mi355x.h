@@ -357,11 +357,12 @@ int fa_launch_paged_append(const void* k, const void* v, const long long* slot_m
  * of one; it only decides how the work is split, any value gives the same
  * result up to rounding. workspace: fa_attention_paged_workspace_bytes of the
  * same numbers on the same device (0: may be NULL); fa_attention_paged_config:
- * the rows of a workgroup and the most chunks a sequence's keys are split into. */
+ * the rows of a workgroup, the wave groups that share its keys and the most chunks
+ * that a sequence's keys are split into. */
 size_t fa_attention_paged_workspace_bytes(int tokens, int num_seqs, int heads, int heads_kv, int head_dim,
                                           int max_query_len, int max_kv_len);
 int fa_attention_paged_config(int tokens, int num_seqs, int heads, int heads_kv, int head_dim, int max_query_len,
-                              int max_kv_len, int* rows_per_block, int* splits);
+                              int max_kv_len, int* rows_per_block, int* kv_groups, int* splits);
 int fa_launch_attention_paged(const void* q, const fa_paged_cache* cache, void* o, void* workspace,
                               size_t workspace_bytes, const int* block_table, const int* query_starts,
                               const int* kv_lens, int num_seqs, int tokens, int heads, int table_width,
@@ -375,7 +376,7 @@ int fa_launch_attention_paged(const void* q, const fa_paged_cache* cache, void* 
  * 128 (else FA_ERROR_UNSUPPORTED). The workspace and the config: as above. */
 size_t fa_attention_cross_workspace_bytes(int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim);
 int fa_attention_cross_config(int batch, int heads, int heads_kv, int q_len, int kv_len, int head_dim,
-                              int* rows_per_block, int* splits);
+                              int* rows_per_block, int* kv_groups, int* splits);
 int fa_launch_attention_cross(const void* q, const void* k, const void* v, void* o, void* workspace,
                               size_t workspace_bytes, const int* kv_lens, int batch, int heads, int heads_kv, int q_len,
                               int kv_len, int head_dim, int dtype, const fa_strides* q_strides,

@@ -210,8 +210,8 @@ def test_paged_splits(fa, dtype, dim, causal):
     for cached, new, heads, heads_kv in (([4000], [1], 4, 2), ([3000, 0, 257, 512, 2047], [1, 1, 1, 1, 1], 8, 1),
                                          ([2500, 100], [70, 40], 2, 1), ([5000], [300], 1, 1), ([2222, 0], [9, 9], 4, 1)):
         b = Paged(fa, cached, new, heads, heads_kv, dim, 16, dtype, seed=7, extra_rows=2)
-        rows, splits = fa.attention_paged_config(b.q.shape[0], len(new), heads, heads_kv, dim, b.max_new, max(b.kv))
-        say("splits", dtype, dim, causal, cached, new, rows, splits)
+        rows, groups, splits = fa.attention_paged_config(b.q.shape[0], len(new), heads, heads_kv, dim, b.max_new, max(b.kv))
+        say("splits", dtype, dim, causal, cached, new, rows, groups, splits)
         assert splits > 1
         b.check(fa, causal, "splits")
         b.check(fa, causal, "splits, long hint", max_kv_len=100000)
@@ -331,6 +331,70 @@ def test_paged_large_scores(fa, dtype):
     b = Paged(fa, [1500, 60], [3, 50], 4, 2, 64, 16, dtype, seed=11, scale=4.0)
     say("large scores", dtype)
     b.check(fa, True, "large scores")
+
+
+# (batch, heads, key heads, new tokens, keys) that take each of the workgroups (rows,
+# wave groups), with and without chunks
+SHAPES = {
+    64: [(200, 4, 4, 1, 33), (4, 16, 16, 1, 1500), (1, 1, 1, 1, 260), (64, 4, 2, 1, 1500), (1, 2, 2, 1000, 90),
+         (1, 1, 1, 1, 33), (1, 1, 1, 1, 700), (3, 10, 5, 301, 533)],
+    128: [(1, 1, 1, 1, 33), (1, 1, 1, 1, 260), (64, 2, 2, 1, 260), (1, 4, 2, 400, 700), (64, 8, 8, 1, 33),
+          (16, 8, 2, 130, 3000), (16, 16, 16, 130, 700), (4, 16, 16, 130, 3000), (16, 1, 1, 1, 260), (2, 1, 1, 1000, 33),
+          (2, 1, 1, 400, 90), (16, 8, 2, 130, 33), (2, 4, 2, 1000, 1500)],
+}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kind", ["paged", "cross"])
+def test_every_configuration(fa, dtype, dim, kind):
+    seen = set()
+    for batch, heads, heads_kv, n, kv in SHAPES[dim]:
+        if kind == "paged":
+            if batch * n * heads * kv > 2e7:
+                continue
+            b = Paged(fa, [kv] * batch, [n] * batch, heads, heads_kv, dim, 16, dtype, seed=n)
+            config = fa.attention_paged_config(batch * n, batch, heads, heads_kv, dim, n, kv + n)
+            say("configuration", kind, dtype, dim, batch, heads, heads_kv, n, kv, config)
+            b.check(fa, True, f"{config}", max_kv_len=kv + n)
+        else:
+            g, t = gen(n), ref.TYPES[dtype]
+            q, k, v = (randn((batch, h, m, dim), t, g) for h, m in ((heads, n), (heads_kv, kv), (heads_kv, kv)))
+            config = fa.attention_cross_config(batch, heads, heads_kv, n, kv, dim)
+            say("configuration", kind, dtype, dim, batch, heads, heads_kv, n, kv, config)
+            out = torch.full_like(q, float("nan"))
+            fa.attention_cross(q, k, v, out=out)
+            torch.cuda.synchronize()
+            want, tol = ref.cross(q, k, v, [kv] * batch)
+            ref.check(out, want, tol, f"cross {config}")
+        seen.add((config[0], config[1], config[2] > 1))
+    say("seen", kind, dim, sorted(seen))
+    rows = {64: [(64, 1), (128, 1), (64, 2)], 128: [(64, 1), (128, 1), (64, 2), (256, 1)]}[dim]
+    assert seen == {(*r, chunks) for r in rows for chunks in (False, True)}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("top", [10, 24, 34])
+def test_paged_one_key_takes_all(fa, dtype, dim, top):
+    """Scores j * 2^top / sqrt(dim) for key j: every row's result is the value of the
+    last key that it sees, exactly, though the base moves at every tile and (from 2^28
+    on) is coarser than the distance of two scores is to a weight."""
+    if dtype == "fp16" and top > 24:
+        top = 24  # j 2^a and 2^b in fp16
+    for new in (1, 70, 200):
+        b = Paged(fa, [240 - new], [new], 2, 1, dim, 16, dtype, seed=new)
+        low = min(top // 2, 6 if dtype == "fp16" else top)
+        b.q[:], b.k[:] = 0, 0
+        b.q[..., 0] = 2.0 ** (top - low) if dtype == "bf16" else 2.0 ** min(top - low, 15)
+        for j in range(240):
+            b.k[b.table[0, j // 16], :, j % 16, 0] = j * 2.0 ** low
+        say("one key", dtype, dim, top, new)
+        for hint in (None, 5000):
+            got = b.run(fa, max_kv_len=hint)
+            last = torch.arange(240 - new, 240, device="cuda")
+            want = b.v[b.table[0].long()[last // 16], 0, last % 16]
+            assert torch.equal(got[:, 0], want) and torch.equal(got[:, 1], want)
 
 
 def _check_not_finite(b, got, causal):

@@ -10,6 +10,7 @@ import torch
 import serving_ref as ref
 
 INVALID = 1  # hipErrorInvalidValue
+CONFIGS = {64: {(64, 1), (128, 1), (64, 2)}, 128: {(64, 1), (128, 1), (64, 2), (256, 1)}}  # (rows, wave groups)
 P = 1 << 20  # a device pointer that nobody follows: every call below is refused
 
 
@@ -76,7 +77,7 @@ def test_paged_refuses_bad_arguments(fa, bad):
 def test_paged_workspace_is_checked(fa):
     sizes = dict(tokens=1, seqs=1, max_q=1, max_kv=8192, width=512, stride=512)
     need = fa.attention_paged_workspace_bytes(1, 1, 8, 4, 64, 1, 8192)
-    rows, splits = fa.attention_paged_config(1, 1, 8, 4, 64, 1, 8192)
+    rows, groups, splits = fa.attention_paged_config(1, 1, 8, 4, 64, 1, 8192)
     assert splits > 1 and need == 8 * splits * (64 + 2) * 4
     for ws, size in ((None, 0), (None, need), (P, need - 1), (P + 8, need)):
         assert refused(fa, paged_status(fa, workspace=ws, workspace_bytes=size, **sizes))
@@ -167,13 +168,13 @@ def test_configurations(fa):
             for seqs, q in ((1, 1), (1, 7), (3, 40), (64, 1), (300, 2), (1, 2048), (8, 512)):
                 for kv in (0, 1, 31, 500, 4096, 70000, 1 << 20, 1 << 30):
                     tokens = seqs * q
-                    rows, splits = fa.attention_paged_config(tokens, seqs, heads, heads_kv, dim, q, kv)
+                    rows, groups, splits = fa.attention_paged_config(tokens, seqs, heads, heads_kv, dim, q, kv)
                     need = fa.attention_paged_workspace_bytes(tokens, seqs, heads, heads_kv, dim, q, kv)
-                    assert rows in (64, 128, 256) and 1 <= splits <= 256
+                    assert (rows, groups) in CONFIGS[dim] and 1 <= splits <= 256
                     assert need == (tokens * heads * splits * (dim + 2) * 4 if splits > 1 else 0)
-                    rows, splits = fa.attention_cross_config(seqs, heads, heads_kv, q, kv, dim)
+                    rows, groups, splits = fa.attention_cross_config(seqs, heads, heads_kv, q, kv, dim)
                     need = fa.attention_cross_workspace_bytes(seqs, heads, heads_kv, q, kv, dim)
-                    assert rows in (64, 128, 256) and 1 <= splits <= 256
+                    assert (rows, groups) in CONFIGS[dim] and 1 <= splits <= 256
                     assert need == (tokens * heads * splits * (dim + 2) * 4 if splits > 1 else 0)
     for bad in ((0, 1, 8, 8, 64, 1, 10), (1, 0, 8, 8, 64, 1, 10), (1, 1, 8, 3, 64, 1, 10), (1, 1, 8, 0, 64, 1, 10),
                 (1, 1, 8, 8, 64, 0, 10), (1, 1, 8, 8, 64, 1, -1)):
