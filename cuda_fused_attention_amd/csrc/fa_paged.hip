@@ -20,7 +20,8 @@ namespace {
 // from the L2) and then writes its share of the slots and the table entries, for
 // which a token looks up its sequence among the sums in LDS. A slot in a new block
 // takes its number from the free list, not from the table, so no workgroup reads
-// what another writes.
+// what another writes. Latency alone: 3.5 us for 8 sequences and for 1000 with 32768
+// new tokens (a launch that does nothing takes about 2).
 struct SlotArgs
 {
     const int* cached;
@@ -154,7 +155,8 @@ int launch_slots(const int* cached, const int* fresh, int num_seqs, int* table, 
 // ------------------------------------------------------------ cache writes
 //
 // One thread moves 16 bytes of a K row and the same 16 of its V row, so a wave has
-// 2 KiB of reads in flight at once. Bound by memory.
+// 2 KiB of reads in flight at once. Bound by memory: 16384 tokens of 8 heads of 128
+// take 27.8 us, 4.83 TB/s (a large copy runs at 4.9); 64 tokens 2.3 us, a launch.
 struct AppendArgs
 {
     const uint16_t* k;

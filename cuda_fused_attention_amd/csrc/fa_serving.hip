@@ -13,9 +13,21 @@
 // r of a sequence is token r / group and head r % group of the key head, so K and
 // V are read once for all of them. A workgroup owns 32 * kWaves rows of one key
 // head (a wave owns 32) and walks 32-key tiles that its waves copy HBM -> LDS
-// together. Few rows over many keys leave the device idle, so the keys of a row
-// block are split into chunks over workgroups; their partial results (O, base, sum
-// in 32 bits) are joined by a second kernel.
+// together; with one new token only one wave has rows, and the others only copy.
+// Few rows over many keys leave the device idle, so the keys of a row block are
+// split into chunks over workgroups; their partial results (O, base, sum in 32 bits)
+// are joined by a second kernel (3.5-7 us of a call's time). Two wave groups of a
+// workgroup can take half of its keys each and meet in LDS, which spares the join.
+//
+// Measured on one MI355X, back to back (a large copy runs at 4.9 TB/s here, a large
+// bf16 matrix product at 1.16-1.21 PFLOP/s):
+//   64 sequences decode over 512 to 8192 keys, 32 heads on 8, dim 128: 220-228 us for
+//   1.14 GB, 5.0-5.2 TB/s: bound by reading K and V;
+//   2048 new tokens over 30720 cached, 32 heads on 8, dim 128: 876 us, 1.22 PFLOP/s, and
+//   (4,8,2048) queries on 8192 states, dim 128: 230-237 us, 1.16-1.19 PFLOP/s: bound by
+//   the matrix cores and the LDS reads of their operands, as the fused forward is;
+//   one sequence, 8 heads, 2049 keys, dim 64: 9.1 us, all latency: 5.7 in the attention
+//   kernel (2.1 until the first tile has come, 0.58 a step), 3.8 in the join.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -407,8 +419,12 @@ __device__ __forceinline__ bool take_block(const Args& a, Block& b, int& split)
 {
     const int head = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.heads_kv));
     const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.heads_kv));
-    // Late rows see the most keys: they start first. First chunks, which every block
-    // has, before second ones: the slots alternate over the XCDs that a head has.
+    // The heads lie next to each other in the grid, so where 8 divides their number all
+    // blocks of a head run on one XCD and share its L2. Late rows see the most keys:
+    // they start first. First chunks, which every block has, come before second ones: a
+    // head of four has two XCDs, over which the slots alternate (chunk by chunk, the
+    // chunks did, and the first ones of short sequences met on one: 76 us against 54 for
+    // four chunks beside 29 decoding sequences).
     split = rest / a.slots;
     return find_block<R, kPaged>(a, a.slots - 1 - rest % a.slots, head, b) && split < b.splits;
 }
@@ -485,11 +501,14 @@ __device__ __forceinline__ void walk(int count, int plain, Step&& step)
     }
 }
 
-// Many rows (128 or 256 of a key head): bound by the matrix cores, beside which
-// the exponentials have to hide. The step of the fused self-attention kernel: in
-// block A the matrix cores compute tile j+1's scores while the vector unit ends
-// tile j's exponentials; past the step's one barrier, in block B, they add tile j's
-// P V while the vector unit starts tile j+1's. K is copied three tiles ahead, V two.
+// The step is the fused self-attention kernel's: in block A the matrix cores compute
+// tile j+1's scores while the vector unit ends tile j's exponentials; past the step's
+// one barrier, in block B, they add tile j's P V while the vector unit starts tile
+// j+1's. K is copied three tiles ahead, V two. A lone wave per SIMD takes 0.60 us a
+// step at head_dim 128 and 0.45 at 64 (its instructions in order), two 0.86 and 0.55:
+// hence 256 rows of 8 waves where there are as many (head_dim 128: the 2048 x 32768
+// chunk 876 us, 128 rows 1005-1116), and more than one workgroup on a CU else. (One
+// tile a step without this overlap took 1251 us for that chunk.)
 // The base is not followed tile by tile: it is set by the first tile and moved only
 // when a tile's row sum passes kSumLimit, which bounds every weight (2^48 in bf16;
 // 2^15 in fp16, whose largest value is near 2^16). The move is rare; it recomputes
@@ -508,7 +527,8 @@ constexpr int kGroupsPerCu = 160 * 1024 / (kGroups * 6 * kTileKeys * D * 2);
 
 template <typename T, int D, int kWaves, int kGroups, bool kPaged>
 __global__ __launch_bounds__(64 * kWaves * kGroups)
-__attribute__((amdgpu_waves_per_eu(kWaves * kGroups > 2 && kGroupsPerCu<D, kGroups> > 1 ? 2 : 1, 8))) void serving_attention_kernel(const Args a)
+__attribute__((amdgpu_waves_per_eu(kWaves * kGroups > 2 && kGroupsPerCu<D, kGroups> > 1 ? 2 : 1, 8))) void
+serving_attention_kernel(const Args a)
 {
     using E = Elem<T>;
     using x8 = typename E::x8;

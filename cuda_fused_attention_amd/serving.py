@@ -213,6 +213,11 @@ def _strides_of(x, name: str):
     return (stride[0] if shape[0] > 1 else dim, stride[1] if shape[1] > 1 else dim, stride[2] if shape[2] > 1 else dim)
 
 
+def _strides_arg(x, name: str):
+    """The strides as a C entry point takes them: none for a contiguous tensor."""
+    return None if x.is_contiguous() else ctypes.byref(_fa.Strides(*_strides_of(x, name)))
+
+
 def _like_q(out, q):
     if out.dtype is not q.dtype or out.shape != q.shape or out.device != q.device:
         raise ValueError("out must have q's shape, type and device")
@@ -308,7 +313,7 @@ def paged_append(k, v, slot_map, cache: PagedCache) -> None:
             or v.device != device):
         raise ValueError(f"k and v must be {dtype} tensors {list(shape)} on {device}")
     status = _lib.fa_launch_paged_append(k.data_ptr(), v.data_ptr(), slot_map.data_ptr(), cache.ref, tokens,
-                                         _strides(_strides_of(k, "k")), _strides(_strides_of(v, "v")), _raw_stream(index))
+                                         _strides_arg(k, "k"), _strides_arg(v, "v"), _raw_stream(index))
     if status:
         raise _fa.FaError(status, "fa_launch_paged_append")
 
@@ -364,7 +369,7 @@ def attention_paged(q, cache: PagedCache, block_table, query_starts, kv_lens, ma
     status = _lib.fa_launch_attention_paged(
         q.data_ptr(), cache.ref, out.data_ptr(), None if room is None else room.data_ptr(), have, block_table.data_ptr(),
         query_starts.data_ptr(), kv_lens.data_ptr(), num_seqs, tokens, heads, width, stride, max_query_len, max_kv_len,
-        1 if causal else 0, _strides(_strides_of(q, "q")), _strides(_strides_of(out, "out")), _raw_stream(index))
+        1 if causal else 0, _strides_arg(q, "q"), _strides_arg(out, "out"), _raw_stream(index))
     if status:
         need = attention_paged_workspace_bytes(tokens, num_seqs, heads, cache.heads_kv, head_dim, max_query_len, max_kv_len)
         _refused(status, "fa_launch_attention_paged", head_dim, workspace, have, need)
@@ -418,8 +423,8 @@ def attention_cross(q, k, v, kv_lens=None, out=None, workspace=None):
     status = _lib.fa_launch_attention_cross(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if room is None else room.data_ptr(), have,
         None if kv_lens is None else kv_lens.data_ptr(), batch, heads, heads_kv, q_len, kv_len, head_dim, _dtype_id(dtype),
-        _strides(_strides_of(q, "q")), _strides(_strides_of(k, "k")), _strides(_strides_of(v, "v")),
-        _strides(_strides_of(out, "out")), _raw_stream(index))
+        _strides_arg(q, "q"), _strides_arg(k, "k"), _strides_arg(v, "v"),
+        _strides_arg(out, "out"), _raw_stream(index))
     if status:
         need = attention_cross_workspace_bytes(batch, heads, heads_kv, q_len, kv_len, head_dim)
         _refused(status, "fa_launch_attention_cross", head_dim, workspace, have, need)
