@@ -282,9 +282,10 @@ int fa_mfma_peak(const void* operands, int mfma_per_wave, int launches, void* re
  * stream the launch goes. A call returns as the launchers above do; refused on
  * the host with hipErrorInvalidValue are also: bases off a 16-byte boundary,
  * strides that are no multiple of 8 elements, key rows closer than head_dim or
- * 2^26 elements or more apart, heads no multiple of heads_kv or above 65536,
- * more than 2^30 keys of a sequence or rows (queries times heads per key head)
- * of one, and a workspace that is missing or too small. */
+ * 2^26 elements or more apart, pages longer than 2^30 elements or more than 2^34
+ * apart, heads no multiple of heads_kv or above 65536, more than 2^30 keys of a
+ * sequence or rows (queries times heads per key head) of one, and a workspace
+ * that is missing or too small. */
 #define FA_DTYPE_BF16 0
 #define FA_DTYPE_FP16 1
 
