@@ -621,6 +621,90 @@ def test_streams_and_repeats(fa):
     say("streams")
 
 
+def test_two_streams_at_once(fa):
+    """Calls that overlap, each with a workspace of its own or one that it allocates."""
+    batches = [Paged(fa, [2500 + 100 * i, 30], [1, 20 + i], 4, 1, 64, 16, "bf16", seed=i) for i in range(4)]
+    alone = [b.run(fa) for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    outs = [torch.full_like(b.q, float("nan")) for b in batches]
+    args = [(ints(b.starts), ints(b.kv)) for b in batches]
+    torch.cuda.synchronize()
+    say("two streams")
+    for _ in range(5):
+        for b, s, o, (starts, kv) in zip(batches, streams, outs, args):
+            with torch.cuda.stream(s):
+                fa.attention_paged(b.q, b.cache, b.table, starts, kv, b.max_new, out=o)
+    torch.cuda.synchronize()
+    for a, o in zip(alone, outs):
+        assert torch.equal(a.view(torch.int16), o.view(torch.int16))
+
+
+def test_cross_in_a_graph(fa):
+    """A captured call follows its tensors' values and lengths; two graphs with a
+    workspace each."""
+    g = gen(4)
+    q, k, v = (randn((4, 2, n, 64), torch.bfloat16, g) for n in (1, 2000, 2000))
+    lens = ints([2000, 1, 700, 0])
+    graphs = []
+    side = torch.cuda.Stream()
+    for _ in range(2):
+        out, ws = torch.empty_like(q), fa.attention_cross_workspace(q, k)
+        assert ws is not None
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            fa.attention_cross(q, k, v, lens, out=out, workspace=ws)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            fa.attention_cross(q, k, v, lens, out=out, workspace=ws)
+        graphs.append((graph, out, ws))
+    for now in ([2000, 1, 700, 0], [5, 2000, 0, 1999], [0, 0, 0, 0], [33, 32, 31, 64]):
+        lens.copy_(ints(now))
+        q.copy_(randn(q.shape, torch.bfloat16, g))
+        eager = fa.attention_cross(q, k, v, lens)
+        torch.cuda.synchronize()
+        say("cross graph", now)
+        for graph, out, ws in graphs:
+            out.fill_(float("nan"))
+            ws.fill_(255)
+            torch.cuda.synchronize()
+            graph.replay()
+        torch.cuda.synchronize()
+        want, tol = ref.cross(q, k, v, now)
+        ref.check(eager, want, tol, "eager")
+        for _, out, _ in graphs:
+            assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
+
+
+@pytest.mark.parametrize("heads,new", [(2, 1), (2, 5), (40, 3)])
+def test_paged_long_cache(fa, heads, new):
+    """300000 cached tokens, as many chunks as a join takes."""
+    b = Paged(fa, [300000], [new], heads, 1, 64, 1024, "bf16", seed=3)
+    say("long cache", heads, new, fa.attention_paged_config(new, 1, heads, 1, 64, new, b.kv[0]))
+    b.check(fa, True, "long cache")
+
+
+@pytest.mark.parametrize("dim,heads,heads_kv,block", [(64, 100, 1, 16), (128, 64, 1, 2048), (64, 36, 2, 64)])
+def test_paged_wide_groups(fa, dim, heads, heads_kv, block):
+    """More query heads on a key head than a wave has rows."""
+    for cached, new in (([70, 5], [1, 3]), ([0, 200], [40, 9]), ([1300], [2])):
+        say("wide groups", dim, heads, heads_kv, block, cached, new)
+        Paged(fa, cached, new, heads, heads_kv, dim, block, "bf16", seed=heads).check(fa, True, "wide groups")
+
+
+def test_paged_thousands_of_sequences(fa):
+    """More sequences than two rounds of the search tell apart."""
+    import random
+
+    rng = random.Random(8)
+    new = [rng.choice([0, 1, 2, 40]) for _ in range(4300)]
+    cached = [rng.choice([0, 3, 20]) for _ in new]
+    say("thousands of sequences")
+    b = Paged(fa, cached, new, 4, 1, 64, 16, "bf16", seed=8, extra_rows=9)
+    b.check(fa, True, "thousands of sequences")
+
+
 def test_refusals(fa):
     b = Paged(fa, [10], [2], 4, 2, 64, 16, "bf16")
     starts, kv = ints(b.starts), ints(b.kv)
