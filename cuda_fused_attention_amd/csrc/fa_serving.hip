@@ -1109,6 +1109,14 @@ constexpr Costs kCosts128 = {{{2, 1, 3, 3.076f, 0.527f, 0.301f},
 constexpr int kSplitChoices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 static_assert(kSplitChoices[15] == kMaxSplits, "the joins' limit");
 
+// Workgroups of the join per row block of `block_rows` rows.
+int join_parts(int block_rows)
+{
+    return block_rows <= kAloneRows ? block_rows : (block_rows + kJoinRows - 1) / kJoinRows;
+}
+
+constexpr double kMaxThreads = 2147483647.0;  // of a launch
+
 Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int head_dim, int max_queries, int max_keys,
                bool paged)
 {
@@ -1147,6 +1155,9 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
             if (choice > 1 && (chunk < 2 || chunk == last_chunk)) continue;
             last_chunk = chunk;
             const int splits = chunk > 0 ? (tiles + chunk - 1) / chunk : 1;
+            if (splits > 1 && (blocks * splits * 64 * c.waves * c.groups > kMaxThreads ||
+                               blocks * join_parts(static_cast<int>(std::min<long long>(rows, R))) * 256 > kMaxThreads))
+                continue;
             auto step_at = [&](double k) {
                 return std::max<double>(c.step, c.shared * std::min<double>(std::max(k, 1.0), c.per_cu));
             };
@@ -1191,7 +1202,7 @@ int launch_typed(const Args& a, const Plan& p, int head_rows, hipStream_t stream
     if (blocks > 0x7fffffffLL / (64 * kWaves * kGroups)) return hipErrorInvalidValue;
     const int block_rows = std::min(32 * kWaves, head_rows);
     const bool alone = block_rows <= kAloneRows;
-    const int parts = alone ? block_rows : (block_rows + kJoinRows - 1) / kJoinRows;
+    const int parts = join_parts(block_rows);
     const long long join_blocks = p.slots * a.heads_kv * parts;
     if (p.splits > 1 && join_blocks > 0x7fffffffLL / 256) return hipErrorInvalidValue;
     const hipError_t e = fa::launch_kernel(serving_attention_kernel<T, D, kWaves, kGroups, kPaged>,

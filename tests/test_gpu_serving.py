@@ -281,6 +281,26 @@ def test_paged_many_sequences(fa, causal):
         Paged(fa, cached, new, 4, 1, 64, 16, "bf16", seed=seqs, extra_rows=7).check(fa, causal, "many sequences")
 
 
+def test_paged_rows_before_the_first_sequence(fa):
+    """Starts that begin past 0: the rows before them belong to no sequence."""
+    for new in ([1, 1, 1], [70, 3, 200], [5, 0, 1]):
+        b = Paged(fa, [9, 40, 0], new, 4, 2, 64, 16, "bf16", extra_rows=80)
+        b.starts = [x + 77 for x in b.starts]
+        say("starts past 0", new)
+        b.check(fa, True, "starts past 0")
+
+
+def test_paged_in_place(fa):
+    """O over q: a workgroup writes the rows that it alone has read."""
+    for cached, new in (([30, 200], [90, 1]), ([3000], [2])):
+        b = Paged(fa, cached, new, 4, 2, 64, 16, "bf16")
+        q = b.q.clone()
+        say("in place", cached, new)
+        got = b.run(fa, out=b.q)
+        want, tol, _ = ref.paged(q, b.k, b.v, b.table, b.starts, b.kv, 16, True)
+        ref.check(got, want, tol, "in place")
+
+
 def test_paged_views(fa):
     """Strided q and out, a wide table's columns, a cache between other data."""
     b = Paged(fa, [30, 0, 77], [5, 40, 1], 4, 2, 64, 16, "bf16", "NHD", extra_rows=1)

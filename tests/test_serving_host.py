@@ -184,6 +184,28 @@ def test_configurations(fa):
     fa.get_last_error()
 
 
+def test_chunks_stay_within_the_grid(fa):
+    """Launches so large that chunks would pass the grid's limit take none."""
+    for seqs, heads, kv in ((1 << 16, 128, 4096), (1 << 17, 64, 1 << 20), (200000, 32, 70000)):
+        rows, groups, splits = fa.attention_paged_config(seqs, seqs, heads, heads, 128, 1, kv)
+        assert seqs * heads * splits * rows * 2 * groups <= 2 ** 31 - 1
+        assert splits == 1 or seqs * heads * 256 <= 2 ** 31 - 1
+        rows, groups, splits = fa.attention_cross_config(seqs, heads, heads, 1, kv, 128)
+        assert seqs * heads * splits * rows * 2 * groups <= 2 ** 31 - 1
+
+
+def test_header_is_plain_c(tmp_path):
+    import os
+    import subprocess
+
+    src = tmp_path / "caller.c"
+    src.write_text('#include "fa_mi355x.h"\n'
+                   "int main(void) { fa_paged_cache c = {0}; fa_strides s = {0, 64, 128}; c.dtype = FA_DTYPE_FP16;\n"
+                   "  return fa_launch_paged_append(0, 0, 0, &c, 0, &s, &s, 0); }\n")
+    include = os.path.join(os.path.dirname(__file__), "..", "include")
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Wextra", "-Werror", "-fsyntax-only", f"-I{include}", str(src)], check=True)
+
+
 def test_structs_match_the_header(fa):
     """The ctypes mirrors have the header's fields in the header's order."""
     import os
