@@ -577,7 +577,7 @@ serving_attention_kernel(const Args a)
         uint32_t koff[kI], voff[kI];  // a copy's lanes: row and chunk from the half's first row
 
         {
-            const int sub = (lane % C::kLanes) / C::kChunks;
+            const int sub = lane / C::kChunks;
             const int pchunk = lane % C::kChunks;
 #pragma unroll
             for (int u = 0; u < kI; ++u)
@@ -604,19 +604,15 @@ serving_attention_kernel(const Args a)
             for (int x = 0; x < kHalves; ++x) p.half[x] = keys.half_at(t * kTileKeys + half0 + 16 * x, pages[x]);
             return p;
         };
-        auto copy = [&](i32x4 d, uint32_t off, uint32_t at) {
-            if constexpr (C::kLanes == 64) fa::dma16(d, off, at);
-            else if (lane < C::kLanes) fa::dma16(d, off, at);
-        };
         auto copy_k = [&](const Place& p, int stage, int u) {
             const auto& half = p.half[kHalves == 1 ? 0 : (u * kWaves * C::kRows) >> 4];
-            copy(keys.descriptor(half.k, half.k_bytes), koff[u],
-                 lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
+            fa::dma16(keys.descriptor(half.k, half.k_bytes), koff[u],
+                      lds_base + stage * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
         };
         auto copy_v = [&](const Place& p, int stage, int u) {
             const auto& half = p.half[kHalves == 1 ? 0 : (u * kWaves * C::kRows) >> 4];
-            copy(keys.descriptor(half.v, half.v_bytes), voff[u],
-                 lds_base + (kStages + stage) * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
+            fa::dma16(keys.descriptor(half.v, half.v_bytes), voff[u],
+                      lds_base + (kStages + stage) * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
         };
         static_assert(kHalves == 1 || 16 % (kWaves * C::kRows) == 0, "every wave's copy u lies in the same half");
 
@@ -1128,6 +1124,7 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
     const bool ragged = paged && seqs > 1;
     const double filled = ragged ? costs.filled : 1.0;
     const double read = static_cast<double>(seqs) * tiles * kTileKeys * heads_kv * head_dim * 4.0 * filled / costs.bytes_per_us;
+    const double read4 = read * read * read * read;
     Plan best{};
     double best_time = 0.0;
     for (int x = 0; x < costs.count; ++x)
@@ -1178,10 +1175,14 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
                 busy = rounds * (c.workgroup + step_at(c.per_cu) * steps) +
                        (rest > 0.0 ? c.workgroup + step_at(rest / cus) * steps : 0.0);
             }
+            const double fixed =
+                costs.launch + (splits > 1 ? costs.join + costs.join_mb * 1e-6 * static_cast<double>(tokens) * heads *
+                                                              head_dim * splits
+                                           : 0.0);
+            if (best_time > 0.0 && busy + fixed >= best_time) continue;
             // A smooth maximum: one of the two hides little of the other where they are close.
-            const double busy2 = busy * busy, read2 = read * read;
-            double time = std::sqrt(std::sqrt(busy2 * busy2 + read2 * read2)) + costs.launch;
-            if (splits > 1) time += costs.join + costs.join_mb * 1e-6 * static_cast<double>(tokens) * heads * head_dim * splits;
+            const double busy2 = busy * busy;
+            const double time = std::sqrt(std::sqrt(busy2 * busy2 + read4)) + fixed;
             if (best_time == 0.0 || time < best_time)
             {
                 best_time = time;

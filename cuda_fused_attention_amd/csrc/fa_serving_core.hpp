@@ -88,16 +88,14 @@ __device__ __forceinline__ int swz_v(int row)
     return D == 128 ? (2 * (row & 3) + 8 * (row & 1)) : (2 * (row & 3));
 }
 
-// How kWaves waves share the copies of a K or V tile: 1 KiB each (64 lanes x
-// 16 bytes), or 512 bytes from the low 32 lanes where a tile has fewer 1 KiB
-// pieces than the workgroup has waves.
+// How kWaves waves share the copies of a K or V tile: 1 KiB each, 64 lanes of 16
+// bytes.
 template <int D, int kWaves>
 struct TileCopy
 {
     static constexpr int kChunks = D / 8;  // 16-byte chunks per row
-    static constexpr int kLanes = kTileKeys * D * 2 / 1024 >= kWaves ? 64 : 32;
-    static constexpr int kBytes = 16 * kLanes;
-    static constexpr int kRows = kLanes / kChunks;                 // rows one copy covers
+    static constexpr int kBytes = 1024;
+    static constexpr int kRows = 64 / kChunks;                     // rows one copy covers
     static constexpr int kIssues = kTileKeys / (kRows * kWaves);  // copies per wave and tile
     static_assert(kIssues >= 1 && kIssues * kRows * kWaves == kTileKeys, "a tile splits evenly over the waves");
     static_assert(16 % kRows == 0, "a copy lies in one half of the tile");
