@@ -21,7 +21,7 @@
 //
 // Measured on one MI355X, back to back (a large copy runs at 4.9 TB/s here, a large
 // bf16 matrix product at 1.16-1.21 PFLOP/s):
-//   64 sequences decode over 512 to 8192 keys, 32 heads on 8, dim 128: 220-228 us for
+//   64 sequences decode over 512 to 8192 keys, 32 heads on 8, dim 128: 220-230 us for
 //   1.14 GB, 5.0-5.2 TB/s: bound by reading K and V;
 //   2048 new tokens over 30720 cached, 32 heads on 8, dim 128: 876 us, 1.22 PFLOP/s, and
 //   (4,8,2048) queries on 8192 states, dim 128: 230-237 us, 1.16-1.19 PFLOP/s: bound by
@@ -523,7 +523,7 @@ constexpr float kCoarseBase = 268435456.0f;
 
 // Workgroups of a CU that the stages leave room for.
 template <int D, int kGroups>
-constexpr int kGroupsPerCu = 160 * 1024 / (kGroups * 6 * kTileKeys * D * 2);
+constexpr int kGroupsPerCu = 160 * 1024 / (kGroups * (D == 128 && kGroups == 2 ? 5 : 6) * kTileKeys * D * 2);
 
 template <typename T, int D, int kWaves, int kGroups, bool kPaged>
 __global__ __launch_bounds__(64 * kWaves * kGroups)
@@ -534,13 +534,16 @@ serving_attention_kernel(const Args a)
     using x8 = typename E::x8;
     using C = TileCopy<D, kWaves>;
     constexpr int R = 32 * kWaves;
-    constexpr int kStages = 3;  // per tensor; four measured no faster
-    static_assert(6 % kStages == 0, "the walk's rounds");
+    // LDS stages: three per tensor (four measured no faster). Two groups at head_dim 128
+    // keep two of K, so that two workgroups fit a CU: K is then copied in block B.
+    constexpr int kKStages = D == 128 && kGroups == 2 ? 2 : 3;
+    constexpr int kVStages = 3;
+    static_assert(6 % kKStages == 0 && 6 % kVStages == 0, "the walk's rounds");
     constexpr int kTile = kTileKeys * D;  // elements
     constexpr int kI = C::kIssues;
     // A wave's copies of a tile lie in one half of it, or in both.
     constexpr int kHalves = kI > 1 ? 2 : 1;
-    constexpr int kGroupElems = 2 * kStages * kTile;
+    constexpr int kGroupElems = (kKStages + kVStages) * kTile;
     // At the end the stages' room holds the second group's results (two groups) and
     // 4 KiB a wave for the stores.
     constexpr int kOtFloats = (D / 32) * 16 * 64;  // one wave's O^T
@@ -575,7 +578,6 @@ serving_attention_kernel(const Args a)
         const Keys<D, kPaged> keys(a, b);
         const float c_log2 = a.c_log2;
         uint32_t koff[kI], voff[kI];  // a copy's lanes: row and chunk from the half's first row
-
         {
             const int sub = lane / C::kChunks;
             const int pchunk = lane % C::kChunks;
@@ -612,7 +614,7 @@ serving_attention_kernel(const Args a)
         auto copy_v = [&](const Place& p, int stage, int u) {
             const auto& half = p.half[kHalves == 1 ? 0 : (u * kWaves * C::kRows) >> 4];
             fa::dma16(keys.descriptor(half.v, half.v_bytes), voff[u],
-                      lds_base + (kStages + stage) * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
+                      lds_base + (kKStages + stage) * (kTile * 2) + (u * kWaves + wave) * C::kBytes);
         };
         static_assert(kHalves == 1 || 16 % (kWaves * C::kRows) == 0, "every wave's copy u lies in the same half");
 
@@ -621,9 +623,9 @@ serving_attention_kernel(const Args a)
         const int lw = r.t_last - t0 - 1;             // last step this wave computes
         const int j_mask = min(lw, r.t_mask - t0 - 1);  // first step whose next tile is masked
 
-        // Prologue: K 0, then K x + 1 and V x in the order of their use. `ahead` is the
-        // place of tile kStages (K next, V a step later), `behind` that of the tile
-        // before it (V next).
+        // Prologue: K 0, then K 1, V 0, K 2, V 1 in the order of their use (two stages of
+        // K: K 2 follows when K 0 has been read). `ahead` is the place of tile 3 (K next,
+        // V a step later), `behind` that of tile 2 (V next).
         Place ahead, behind;
         fetch_pages(t0);
         behind = place_of(t0);
@@ -631,18 +633,19 @@ serving_attention_kernel(const Args a)
 #pragma unroll
         for (int u = 0; u < kI; ++u) copy_k(behind, 0, u);
 #pragma unroll
-        for (int x = 1; x < kStages; ++x)
+        for (int x = 1; x < 3; ++x)
         {
             ahead = place_of(t0 + x);
             fetch_pages(t0 + x + 1);
 #pragma unroll
-            for (int u = 0; u < kI; ++u) copy_k(ahead, x, u);
+            for (int u = 0; u < kI; ++u)
+                if (x < kKStages) copy_k(ahead, x, u);
 #pragma unroll
             for (int u = 0; u < kI; ++u) copy_v(behind, x - 1, u);
             behind = ahead;
         }
-        ahead = place_of(t0 + kStages);
-        fetch_pages(t0 + kStages + 1);
+        ahead = place_of(t0 + 3);
+        fetch_pages(t0 + 4);
 
         x8 qr[D / 16];
         const uint16_t* qp = a.q + q_offset<kPaged>(a, b, r);
@@ -653,7 +656,7 @@ serving_attention_kernel(const Args a)
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) k_at[ks] = 2 * (grp * kGroupElems + k_read_offset<D>(i, h, ks));
 #pragma unroll
-        for (int db = 0; db < D / 32; ++db) v_at[db] = 2 * (grp * kGroupElems + kStages * kTile + v_read_offset<D>(lane, db));
+        for (int db = 0; db < D / 32; ++db) v_at[db] = 2 * (grp * kGroupElems + kKStages * kTile + v_read_offset<D>(lane, db));
         x8 ka[D / 16], va[D / 32][2];
         auto load_k = [&](int stage, int first, int count) {
 #pragma unroll
@@ -682,8 +685,8 @@ serving_attention_kernel(const Args a)
             if (__any(base != kEmptyBase && __builtin_fabsf(base) >= kCoarseBase)) limit_bits = __builtin_bit_cast(int, -1.0f);
             limit_bits = uniform(limit_bits);
         };
-        // K 0 has landed: kStages - 1 tiles of K and of V may fly.
-        fa::wait_vm_lgkm0<2 * (kStages - 1) * kI>();
+        // K 0 has landed: the other tiles of K and of V may fly.
+        fa::wait_vm_lgkm0<(kKStages + 1) * kI>();
         barrier();
         if (lw >= 0)
         {
@@ -697,9 +700,12 @@ serving_attention_kernel(const Args a)
             note_base(m);
         }
         // K 1 and V 0 have landed, K 0's stage is free.
-        fa::wait_vm_lgkm0<(2 * kStages - 4) * kI>();
+        fa::wait_vm_lgkm0<(kKStages - 1) * kI>();
         barrier();
         load_k(1, 0, D / 16);
+        if constexpr (kKStages == 2)
+#pragma unroll
+            for (int u = 0; u < kI; ++u) copy_k(behind, 0, u);
 
         // A weight of 0 times an infinity or a NaN is NaN. A tile that some lane does not
         // see whole (at most two of a wave: its rows' limits lie within 32 keys) is left
@@ -746,7 +752,7 @@ serving_attention_kernel(const Args a)
             weigh<T, true>(st, 0, pr[0], m, c_log2, sum);
             weigh<T, true>(st, 8, pr[1], m, c_log2, sum);
             l = l * alpha + sum;
-            load_v(P % kStages, 0, D / 32);
+            load_v(P % kVStages, 0, D / 32);
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) o[x % (D / 32)] = E::mfma(va[x % (D / 32)][x / (D / 32)], pr[x / (D / 32)], o[x % (D / 32)]);
             tsum = 0.0f;
@@ -786,9 +792,9 @@ serving_attention_kernel(const Args a)
             {
                 qk_part(sbuf[B ^ 1], c * kMfmaPer, 1);
                 __builtin_amdgcn_sched_barrier(0);
-                copy_k(ahead, P % kStages, c);
+                if constexpr (kKStages == 3) copy_k(ahead, P % 3, c);
                 __builtin_amdgcn_sched_barrier(0);
-                load_v(P % kStages, c * kVPer, kVPer);
+                load_v(P % kVStages, c * kVPer, kVPer);
                 qk_part(sbuf[B ^ 1], c * kMfmaPer + 1, kMfmaPer - 1);
                 weigh_part(sbuf[B], 8, p_hi, c * kExpPer);
                 __builtin_amdgcn_sched_barrier(0);
@@ -797,7 +803,7 @@ serving_attention_kernel(const Args a)
             pin(tsum);
             // K jj+2 and V jj+1 have landed (what was issued after them may fly), every
             // LDS read is done.
-            fa::wait_vm_lgkm0<(2 * kStages - 5) * kI>();
+            fa::wait_vm_lgkm0<(kKStages - 2) * kI>();
             barrier();
             // Block B
             bool rare = __any(tsum > __builtin_bit_cast(float, limit_bits));
@@ -828,16 +834,17 @@ serving_attention_kernel(const Args a)
             {
                 pv_part(p_cur, c * kMfmaPer, 1);
                 __builtin_amdgcn_sched_barrier(0);
-                copy_v(behind, (P + kStages - 1) % kStages, c);
+                if constexpr (kKStages == 2) copy_k(ahead, (P + 3) % 2, c);
+                copy_v(behind, (P + 2) % kVStages, c);
                 __builtin_amdgcn_sched_barrier(0);
-                load_k((P + 2) % kStages, c * kKPer, kKPer);
+                load_k((P + 2) % kKStages, c * kKPer, kKPer);
                 pv_part(p_cur, c * kMfmaPer + 1, kMfmaPer - 1);
                 weigh_part(sbuf[B ^ 1], 0, p_lo[B ^ 1], c * kExpPer);
                 __builtin_amdgcn_sched_barrier(0);
             }
             behind = ahead;
-            ahead = place_of(t0 + jj + kStages + 1);
-            fetch_pages(t0 + jj + kStages + 2);
+            ahead = place_of(t0 + jj + 4);
+            fetch_pages(t0 + jj + 5);
             pin8(p_lo[B ^ 1]);
             pin(tsum);
             if (rare) rebase(par_tag, jj);
@@ -848,16 +855,19 @@ serving_attention_kernel(const Args a)
         // The steps past this wave's last tile: its share of the copies and the barriers.
         for (int jj = active; jj < cnt; ++jj)
         {
-            const int stage = jj % kStages;
 #pragma unroll
-            for (int u = 0; u < kI; ++u) copy_k(ahead, stage, u);
-            fa::wait_vm_lgkm0<(2 * kStages - 5) * kI>();
+            for (int u = 0; u < kI; ++u)
+                if constexpr (kKStages == 3) copy_k(ahead, jj % 3, u);
+            fa::wait_vm_lgkm0<(kKStages - 2) * kI>();
             barrier();
 #pragma unroll
-            for (int u = 0; u < kI; ++u) copy_v(behind, (stage + kStages - 1) % kStages, u);
+            for (int u = 0; u < kI; ++u)
+                if constexpr (kKStages == 2) copy_k(ahead, (jj + 3) % 2, u);
+#pragma unroll
+            for (int u = 0; u < kI; ++u) copy_v(behind, (jj + 2) % kVStages, u);
             behind = ahead;
-            ahead = place_of(t0 + jj + kStages + 1);
-            fetch_pages(t0 + jj + kStages + 2);
+            ahead = place_of(t0 + jj + 4);
+            fetch_pages(t0 + jj + 5);
         }
         // The tiles that were left out, a key at a time.
         for (int t = r.t_mask; kPaged && left_out != 0; ++t, left_out >>= 1)
@@ -1075,10 +1085,10 @@ struct Plan
 //                when the other ends). Only the device knows the lengths: their mean
 //                is taken as `filled` of the longest.
 // Not below what reading the keys once takes, plus the join's time. The constants are
-// fits to 1020 drawn shapes (1 to 192 sequences, 1 to 32768 keys, 1 to 64 heads, one
+// fits to 1150 drawn shapes (1 to 192 sequences, 1 to 32768 keys, 1 to 64 heads, one
 // new token to chunks of 4096), each at every rows and chunks of the lists below. The
-// choice takes 1.031 (head_dim 64) and 1.046 (128) times the best one's time in the
-// geometric mean, more than 1.2 times it at 39 of the 1020. Without the two groups it
+// choice takes 1.027 (head_dim 64) and 1.044 (128) times the best one's time in the
+// geometric mean, more than 1.2 times it at 37 of the 1150. Without the two groups it
 // would be 1.038 and 1.064; two groups of 128 rows gain 0.4 % and are not built, and
 // 256 rows are of no use at head_dim 64.
 struct RowsCost
@@ -1097,11 +1107,11 @@ struct Costs
 constexpr Costs kCosts64 = {
     {{2, 1, 6, 2.857f, 0.454f, 0.131f}, {4, 1, 3, 2.849f, 0.365f, 0.151f}, {2, 2, 3, 3.68f, 0.384f, 0.205f}},
     3, 0.9f, 0.507f, 4.118f, 1.335f, 1.95f, 5.958e6f};
-constexpr Costs kCosts128 = {{{2, 1, 3, 3.076f, 0.527f, 0.301f},
-                              {4, 1, 2, 2.753f, 0.749f, 0.285f},
-                              {8, 1, 1, 3.781f, 0.676f, 0.4f},
-                              {2, 2, 1, 3.998f, 0.648f, 0.394f}},
-                             4, 0.9f, 0.601f, 2.864f, 1.855f, 3.612f, 6.901e6f};
+constexpr Costs kCosts128 = {{{2, 1, 3, 3.479f, 0.586f, 0.286f},
+                              {4, 1, 2, 3.318f, 0.551f, 0.392f},
+                              {8, 1, 1, 4.233f, 0.57f, 0.631f},
+                              {2, 2, 2, 3.748f, 0.704f, 0.452f}},
+                             4, 0.852f, 0.44f, 2.596f, 1.533f, 4.251f, 5.109e6f};
 constexpr int kSplitChoices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 static_assert(kSplitChoices[15] == kMaxSplits, "the joins' limit");
 
@@ -1152,9 +1162,12 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
             if (choice > 1 && (chunk < 2 || chunk == last_chunk)) continue;
             last_chunk = chunk;
             const int splits = chunk > 0 ? (tiles + chunk - 1) / chunk : 1;
-            if (splits > 1 && (blocks * splits * 64 * c.waves * c.groups > kMaxThreads ||
-                               blocks * join_parts(static_cast<int>(std::min<long long>(rows, R))) * 256 > kMaxThreads))
-                continue;
+            // Both grids have to hold it; the first choice stands where none fits, and its
+            // launch is refused.
+            const bool fits = blocks * splits * 64 * c.waves * c.groups <= kMaxThreads &&
+                              (splits == 1 ||
+                               blocks * join_parts(static_cast<int>(std::min<long long>(rows, R))) * 256 <= kMaxThreads);
+            if (!fits && best.waves > 0) continue;
             auto step_at = [&](double k) {
                 return std::max<double>(c.step, c.shared * std::min<double>(std::max(k, 1.0), c.per_cu));
             };
@@ -1185,7 +1198,7 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
             const double time = std::sqrt(std::sqrt(busy2 * busy2 + read4)) + fixed;
             if (best_time == 0.0 || time < best_time)
             {
-                best_time = time;
+                best_time = fits ? time : 0.0;
                 best = p;
                 best.splits = splits;
                 best.chunk = std::max(chunk, 1) * kTileKeys;
