@@ -960,10 +960,14 @@ serving_attention_kernel(const Args a)
 
 // Joins the chunks of a row: O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c with
 // M the largest base, kept running. D/4 lanes read a chunk's 4 D bytes, so 256
-// threads make 1024/D groups: for few rows with many chunks (kAlone) they all work on
-// one row, chunk by chunk in turn, and meet in LDS; else each takes rows of its own.
-constexpr int kAloneRows = 16;  // rows of a block up to which each has a workgroup to itself
-constexpr int kJoinRows = 32;  // rows of a workgroup that are not kAlone
+// threads make 1024/D groups. For many chunks they all work on one row, chunk by chunk
+// in turn, and meet in LDS (kAlone); for few each takes rows of its own. A whole call,
+// alone against not: 33 chunks of one row a head 9.0 us against 10.0, 65 chunks of 16
+// rows 16.4 against 26.9, 17 of 36 rows 46.2 against 50.6; 9 of 4 rows (64 sequences)
+// 228.7 against 224.6, 17 chunks of 96 rows the same.
+constexpr int kAloneChunks = 13;  // from this many on
+constexpr int kAloneRows = 64;    // and up to as many rows of a block
+constexpr int kJoinRows = 32;     // rows of a workgroup that are not kAlone
 
 template <typename T, int D, int R, bool kPaged, bool kAlone>
 __global__ __launch_bounds__(256) void serving_join_kernel(const Args a, int block_parts)
@@ -1115,10 +1119,12 @@ constexpr Costs kCosts128 = {{{2, 1, 3, 3.479f, 0.586f, 0.286f},
 constexpr int kSplitChoices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256};
 static_assert(kSplitChoices[15] == kMaxSplits, "the joins' limit");
 
+bool joins_alone(int block_rows, int splits) { return splits >= kAloneChunks && block_rows <= kAloneRows; }
+
 // Workgroups of the join per row block of `block_rows` rows.
-int join_parts(int block_rows)
+int join_parts(int block_rows, int splits)
 {
-    return block_rows <= kAloneRows ? block_rows : (block_rows + kJoinRows - 1) / kJoinRows;
+    return joins_alone(block_rows, splits) ? block_rows : (block_rows + kJoinRows - 1) / kJoinRows;
 }
 
 constexpr double kMaxThreads = 2147483647.0;  // of a launch
@@ -1166,7 +1172,7 @@ Plan make_plan(long long seqs, long long tokens, int heads, int heads_kv, int he
             // launch is refused.
             const bool fits = blocks * splits * 64 * c.waves * c.groups <= kMaxThreads &&
                               (splits == 1 ||
-                               blocks * join_parts(static_cast<int>(std::min<long long>(rows, R))) * 256 <= kMaxThreads);
+                               blocks * join_parts(static_cast<int>(std::min<long long>(rows, R)), splits) * 256 <= kMaxThreads);
             if (!fits && best.waves > 0) continue;
             auto step_at = [&](double k) {
                 return std::max<double>(c.step, c.shared * std::min<double>(std::max(k, 1.0), c.per_cu));
@@ -1215,8 +1221,8 @@ int launch_typed(const Args& a, const Plan& p, int head_rows, hipStream_t stream
     const long long blocks = p.slots * a.heads_kv * p.splits;
     if (blocks > 0x7fffffffLL / (64 * kWaves * kGroups)) return hipErrorInvalidValue;
     const int block_rows = std::min(32 * kWaves, head_rows);
-    const bool alone = block_rows <= kAloneRows;
-    const int parts = join_parts(block_rows);
+    const bool alone = joins_alone(block_rows, p.splits);
+    const int parts = join_parts(block_rows, p.splits);
     const long long join_blocks = p.slots * a.heads_kv * parts;
     if (p.splits > 1 && join_blocks > 0x7fffffffLL / 256) return hipErrorInvalidValue;
     const hipError_t e = fa::launch_kernel(serving_attention_kernel<T, D, kWaves, kGroups, kPaged>,

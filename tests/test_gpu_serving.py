@@ -417,6 +417,23 @@ def test_paged_one_key_takes_all(fa, dtype, dim, top):
             assert torch.equal(got[:, 0], want) and torch.equal(got[:, 1], want)
 
 
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_not_finite_queries(fa, value):
+    """A query row that is not finite makes its own row NaN, and no other."""
+    b = Paged(fa, [40, 1500], [50, 3], 4, 2, 64, 16, "bf16", seed=2)
+    want, tol, _ = ref.paged(b.q, b.k, b.v, b.table, b.starts, b.kv, 16, True)
+    for row, h in ((7, 1), (33, 3), (51, 0)):
+        b.q[row, h, 9] = value
+    say("not finite q", value)
+    for hint in (None, 200):
+        got = b.run(fa, max_kv_len=hint)
+        bad = torch.zeros(got.shape[:2], dtype=torch.bool, device="cuda")
+        for row, h in ((7, 1), (33, 3), (51, 0)):
+            bad[row, h] = True
+        assert got[bad].isnan().all()
+        ref.check(got[~bad], want[~bad], tol[~bad], "other rows")
+
+
 def _check_not_finite(b, got, causal):
     """Rows against sums over the keys that each sees: infinities and NaN where one of
     those holds them, the usual tolerance elsewhere. fp16 weights are multiples of 2^-24
@@ -695,6 +712,17 @@ def test_cross_in_a_graph(fa):
         ref.check(eager, want, tol, "eager")
         for _, out, _ in graphs:
             assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_paged_joins(fa, dim):
+    """Few and many chunks of few and many rows: both ways to join them."""
+    for cached, new, heads, heads_kv in (([800], [1], 2, 2), ([6000], [1], 8, 1), ([6000], [9], 4, 1), ([5000], [20], 6, 1),
+                                         ([900], [30], 2, 1), ([2000, 5], [14, 1], 4, 1)):
+        b = Paged(fa, cached, new, heads, heads_kv, dim, 32, "bf16", seed=len(cached) + new[0])
+        config = fa.attention_paged_config(b.q.shape[0], len(new), heads, heads_kv, dim, b.max_new, max(b.kv))
+        say("joins", dim, cached, new, heads, heads_kv, config)
+        b.check(fa, True, f"joins {config}", max_kv_len=max(b.kv))
 
 
 @pytest.mark.parametrize("heads,new", [(2, 1), (2, 5), (40, 3)])
