@@ -521,13 +521,17 @@ constexpr float kSumLimit<_Float16> = 32768.0f;
 // (fp32's spacing at 2^28 is 32): every tile takes the exact path.
 constexpr float kCoarseBase = 268435456.0f;
 
-// Workgroups of a CU that the stages leave room for.
-template <int D, int kGroups>
-constexpr int kGroupsPerCu = 160 * 1024 / (kGroups * (D == 128 && kGroups == 2 ? 5 : 6) * kTileKeys * D * 2);
+// Waves of a SIMD that the stages leave room for; the registers are kept to as many.
+// Left to itself the compiler took 177 (head_dim 64) and 265 (128) for 64 rows of
+// contiguous keys, and four and two workgroups ran on a CU where six and three fit:
+// 64 x 32 heads of 60 queries on 77 keys take 19.4 us against 21.2 at head_dim 64 and
+// 34.5 against 36.4 at 128, 256 x 32 heads on 512 keys 229 against 238.
+template <int D>
+constexpr int kWavesPerSimd = D == 64 ? 3 : 2;
 
 template <typename T, int D, int kWaves, int kGroups, bool kPaged>
 __global__ __launch_bounds__(64 * kWaves * kGroups)
-__attribute__((amdgpu_waves_per_eu(kWaves * kGroups > 2 && kGroupsPerCu<D, kGroups> > 1 ? 2 : 1, 8))) void
+__attribute__((amdgpu_waves_per_eu(kWavesPerSimd<D>, 8))) void
 serving_attention_kernel(const Args a)
 {
     using E = Elem<T>;
